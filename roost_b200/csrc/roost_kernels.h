@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define ROOST_ABI_VERSION 17
+#define ROOST_ABI_VERSION 18
 
 #define ROOST_OK 0
 #define ROOST_ERR_INVALID 1      /* an argument is out of range or inconsistent; nothing was launched */
@@ -625,6 +625,33 @@ int roost_xielu(const void* x, void* out, int64_t n, float a_pos, float a_neg, i
 int roost_relu_squared(const void* x, void* out, int64_t n, int dtype, roost_stream_t stream);   /* y = max(z, 0)^2 */
 /* x[t, h, :] *= sigmoid(g[t, col + h]) in place; g's rows are ld_g apart. */
 int roost_head_gate_mul(void* x, const void* g, int64_t ld_g, int col, int tokens, int heads, int vdim, int dtype, roost_stream_t stream);
+
+/* ---- rows_e4m3.cu: rows in 8 bits (e4m3) with a scale a row: scale[t] = max(max |v[t, :]| / 448, 2^-126), q[t, i] nearest to v[t, i] / scale[t].
+ * A row that holds an infinity or a NaN has a scale that is not finite and makes the row of a product with it NaN. ---- */
+#define ROOST_E4M3_MAX_COLS 51168   /* the longest row these entry points serve */
+/* v = x; rows ldx elements apart, q contiguous. */
+int roost_quantise_e4m3(const void* x, int64_t ldx, void* q, float* scale, int rows, int cols, int dtype, roost_stream_t stream);
+/* v = silu(gate) * up in 32 bits, x and block as roost_silu_mul. */
+int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tokens, int inter, int block, int dtype, roost_stream_t stream);
+/* v = rms_norm(s) * w in 32 bits with s = x, or residual + x rounded to residual_dtype (that of x, or float32) where residual is not null; s
+ * replaces residual unless `rows` gathers (as roost_add_rms_norm). kept (null, or of x's type): v as the norm without the 8 bits gives it. */
+int roost_rms_norm_e4m3(const void* x, void* residual, const void* w, void* q, float* scale, void* kept, const int32_t* rows, int n_out, int hidden,
+                        float eps, int dtype, int residual_dtype, int wdtype, roost_stream_t stream);
+
+/* ---- gemm_e4m3.cu ---- */
+/* out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k], 32-bit sums, any sizes and strides (in elements). */
+int roost_gemm_e4m3(const void* q, const float* q_scale, const void* w, const float* w_scale, void* out, int m, int n, int k, int64_t ldq, int64_t ldw,
+                    int64_t ldo, int out_dtype, roost_stream_t stream);
+
+/* ---- adapters.cu ---- */
+/* y[t, n] += scales[s] sum_r b[s, n, r] sum_k a[s, p, r, k] x[t, k] for the tokens t of the list, p the part of output n: the parts lie one after the
+ * other, widths (host memory) outputs each. a [slots, n_parts, rank, inputs] and b [slots, outputs, rank] have x's type; the first ranks[s] of a
+ * slot's rows are used (null: all). rows[0 .. listed): the tokens that have an adapter; tiles [n_tiles][3] = (slot, first, end): the tokens
+ * rows[first .. end), at most 64, have adapter `slot`; a slot outside [0, slots) or a token outside [0, tokens) is passed over. A token is listed
+ * once at most. y's other rows are left as they are. n_parts <= 8, n_parts * rank <= 512. */
+int roost_adapters_add(void* y, int64_t ldy, const void* x, int64_t ldx, const void* a, const void* b, const float* scales, const int32_t* ranks,
+                       const int32_t* rows, const int32_t* tiles, int n_tiles, int listed, int tokens, int slots, int n_parts, const int32_t* widths,
+                       int rank, int inputs, int dtype, int y_dtype, roost_stream_t stream);
 
 #ifdef __cplusplus
 }

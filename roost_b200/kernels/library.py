@@ -10,11 +10,12 @@ import ctypes
 from dataclasses import dataclass
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
+import numpy as np
 import torch
 
 from . import build
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 F32, BF16 = 0, 1
 GATE_FUNCTIONS = {"silu": 0, "gelu_tanh": 1, "clamped_swish": 2}   # the codes of csrc/roost_kernels.h
 
@@ -54,6 +55,17 @@ def _need(t: torch.Tensor, name: str, dtype=None):
         raise KernelError(f"{name} is not contiguous")
     if dtype is not None and t.dtype != dtype:
         raise KernelError(f"{name} has dtype {t.dtype}; expected {dtype}")
+
+
+def _need_here(**tensors):
+    """Every tensor given (None: left out) lies on the current device, whose current stream the call goes to."""
+    for name, t in tensors.items():
+        if t is not None and not t.is_cuda:
+            raise KernelError(f"{name} is not on a CUDA device")
+    here = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and t.device.index != here:
+            raise KernelError(f"{name} is on {t.device}; the call goes to the current device, cuda:{here}")
 
 
 def _need_rows(t: torch.Tensor, name: str, dtype=None):
@@ -228,6 +240,12 @@ _SIGNATURES = {
                           c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p],
     "roost_mamba1_scan_chunks": [c_int, c_int],
     "roost_moe_combine": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "roost_quantise_e4m3": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    "roost_silu_mul_e4m3": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "roost_rms_norm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p],
+    "roost_gemm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
+    "roost_adapters_add": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
+                           c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "roost_argmax": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p],
     "roost_argmax_split": [c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "roost_sample": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -254,6 +272,35 @@ class MoeRoute:
     real: int = 1 << 30                        # experts from here on are identity experts: rows without weights
     wide_tiles: torch.Tensor | None = None     # the same rows in tiles of 128, for the tcgen05 product of steps of many rows
     max_wide_tiles: int = 0
+
+
+@dataclass
+class AdapterPlan:
+    """Which tokens of a step have which adapter (``adapter_plan``). ``rows``: the tokens that have one, those of an adapter together;
+    ``tiles`` [n, 3]: (slot, first, end), the tokens ``rows[first:end]`` have that adapter (slot -1: an unused entry); ``tokens``: the step's."""
+    rows: torch.Tensor
+    tiles: torch.Tensor
+    tokens: int
+
+
+ADAPTER_TILE_ROWS = 64   # tokens of a tile of an adapter plan at most
+
+
+def adapter_lists(row_counts: list, row_slots: list) -> tuple:
+    """(rows, tiles) of an ``AdapterPlan`` as int32 numpy arrays, for a step whose i-th request brings ``row_counts[i]`` tokens and uses the adapter
+    in slot ``row_slots[i]`` (negative: none)."""
+    if len(row_counts) != len(row_slots):
+        raise KernelError(f"adapter_plan: {len(row_counts)} requests, {len(row_slots)} adapters")
+    counts, slots = np.asarray(row_counts, np.int64), np.asarray(row_slots, np.int64)
+    if counts.size and counts.min() < 0:
+        raise KernelError("adapter_plan: a request has fewer than no tokens")
+    of = np.repeat(slots, counts)                                   # each token's adapter
+    order = np.argsort(of, kind="stable")
+    rows = order[np.searchsorted(of[order], 0):]                    # tokens without an adapter are left out
+    used, first = np.unique(of[rows], return_index=True)
+    ends = np.append(first[1:], rows.size)
+    tiles = [(s, at, min(at + ADAPTER_TILE_ROWS, end)) for s, lo, end in zip(used, first, ends) for at in range(lo, end, ADAPTER_TILE_ROWS)]
+    return rows.astype(np.int32), np.asarray(tiles, np.int32).reshape(-1, 3)
 
 
 MOE_TCGEN05_MIN_ROWS = 1024  # sorted rows from which a bfloat16 step runs the experts' products on tcgen05
@@ -381,6 +428,103 @@ class KernelLibrary:
         out = torch.empty((M, N // 2), dtype=torch.bfloat16, device=a.device)
         self._call("roost_gemm_tcgen05_swiglu", _ptr(a), _ptr(w), _ptr(out), M, N, K, a.stride(0), w.stride(0), out.stride(0), _stream())
         return out
+
+    # ---- rows in 8 bits. A row v stands as q (e4m3) times scale (float32), scale = max(max |v| / 448, 2^-126) and q nearest to v / scale. A row
+    # that holds an infinity or a NaN makes its row of a product NaN.
+    @staticmethod
+    def _e4m3_rows(shape, device):
+        return torch.empty(shape, dtype=torch.float8_e4m3fn, device=device), torch.empty(shape[:-1], dtype=torch.float32, device=device)
+
+    def quantise_e4m3(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(q, scale) of the rows of x [T, W], which may lie apart: activations ahead of ``gemm_e4m3``, or a weight's rows."""
+        _need_here(x=x); _need_rows(x, "x")
+        T, W = x.shape
+        q, scale = self._e4m3_rows((T, W), x.device)
+        self._call("roost_quantise_e4m3", _ptr(x), x.stride(0) if T > 1 else W, _ptr(q), _ptr(scale), T, W, dtype_code(x.dtype), _stream())
+        return q, scale
+
+    def silu_mul_e4m3(self, x: torch.Tensor, block: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+        """(q, scale) of silu(gate) * up, which is not rounded before; x and ``block`` as ``silu_mul``."""
+        _need_here(x=x); _need(x, "x")
+        if x.dim() != 2 or x.shape[1] % 2:
+            raise KernelError(f"silu_mul_e4m3: x is {tuple(x.shape)}; expected rows of gate and up values")
+        T, inter = x.shape[0], x.shape[1] // 2
+        q, scale = self._e4m3_rows((T, inter), x.device)
+        self._call("roost_silu_mul_e4m3", _ptr(x), _ptr(q), _ptr(scale), T, inter, block, dtype_code(x.dtype), _stream())
+        return q, scale
+
+    def _rms_norm_e4m3(self, x, residual, w, eps, rows, keep):
+        _need_here(x=x, residual=residual, w=w, rows=rows); _need(x, "x"); _need(w, "w")
+        H = x.shape[-1]
+        if w.numel() != H:
+            raise KernelError(f"rms_norm_e4m3: weight has {w.numel()} elements for rows of {H}")
+        if rows is not None:
+            _need(rows, "rows", torch.int32)
+        shape = tuple(x.shape) if rows is None else (rows.numel(), H)
+        q, scale = self._e4m3_rows(shape, x.device)
+        kept = torch.empty(shape, dtype=x.dtype, device=x.device) if keep else None
+        self._call("roost_rms_norm_e4m3", _ptr(x), _ptr(residual), _ptr(w), _ptr(q), _ptr(scale), _ptr(kept), _ptr(rows), scale.numel(), H, eps,
+                   dtype_code(x.dtype), dtype_code(x.dtype if residual is None else residual.dtype), dtype_code(w.dtype), _stream())
+        return (q, scale, kept) if keep else (q, scale)
+
+    def rms_norm_e4m3(self, x: torch.Tensor, w: torch.Tensor, eps: float, rows: torch.Tensor | None = None, keep: bool = False):
+        """(q, scale) of ``rms_norm``'s rows, which are not rounded before; with ``keep`` the norm in x's type as a third result (what the
+        adapters beside the product read)."""
+        return self._rms_norm_e4m3(x, None, w, eps, rows, keep)
+
+    def add_rms_norm_e4m3(self, x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, eps: float, rows: torch.Tensor | None = None, keep: bool = False):
+        """residual += x (in place, unless ``rows`` gathers), rounded to the residual's type (x's, or float32 beside bfloat16), and (q, scale) of
+        the norm of the sum; ``keep`` as ``rms_norm_e4m3``."""
+        _need(residual, "residual")
+        if residual.shape != x.shape:
+            raise KernelError("add_rms_norm_e4m3: x and residual do not agree in shape")
+        return self._rms_norm_e4m3(x, residual, w, eps, rows, keep)
+
+    def gemm_e4m3(self, q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k] for rows in 8 bits on either side (``quantise_e4m3`` and its like), 32-bit sums."""
+        _need_here(q=q, q_scale=q_scale, w=w, w_scale=w_scale)
+        _need_rows(q, "q", torch.float8_e4m3fn); _need_rows(w, "w", torch.float8_e4m3fn)
+        _need(q_scale, "q_scale", torch.float32); _need(w_scale, "w_scale", torch.float32)
+        (M, K), (N, K2) = q.shape, w.shape
+        if K != K2 or q_scale.numel() != M or w_scale.numel() != N:
+            raise KernelError(f"gemm_e4m3: q {tuple(q.shape)}, w {tuple(w.shape)} and scales of {q_scale.numel()} and {w_scale.numel()} rows do not agree")
+        out = torch.empty((M, N), dtype=out_dtype, device=q.device)
+        self._call("roost_gemm_e4m3", _ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), _ptr(out), M, N, K, q.stride(0) if M > 1 else K,
+                   w.stride(0) if N > 1 else K, N, dtype_code(out_dtype), _stream())
+        return out
+
+    # ---- adapters
+    def adapter_plan(self, row_counts: list, row_slots: list, device=None) -> AdapterPlan:
+        """The lists by which ``adapters_add_`` deals a step's tokens out, for all the step's layers: request i brings ``row_counts[i]`` tokens, one
+        request after the other, and uses the adapter in slot ``row_slots[i]`` (negative: none)."""
+        rows, tiles = adapter_lists(row_counts, row_slots)
+        both = torch.from_numpy(np.concatenate([tiles.reshape(-1), rows])).to(device if device is not None else "cuda")
+        return AdapterPlan(rows=both[tiles.size:], tiles=both[:tiles.size].view(-1, 3), tokens=int(sum(row_counts)))
+
+    def adapters_add_(self, y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, plan: AdapterPlan,
+                      widths: tuple | None = None, ranks: torch.Tensor | None = None) -> torch.Tensor:
+        """y[t] += scale[s] * b[s] (a[s] x[t]) in place for every token t whose request has an adapter s; the other rows of y stay as they are. y: what
+        the shared projection made of x, rows [T, N] that may lie apart, in x's type (or float32 beside bfloat16). ``widths``: the parts of the
+        projection's outputs (queries, keys and values, say), each with an adapter of its own; None: one part. a [slots, parts, rank, K] and b
+        [slots, N, rank] in x's type, scale float32 [slots]; ``ranks`` int32 [slots]: how many of the rank's rows a slot uses (None: all)."""
+        _need_here(y=y, x=x, a=a, b=b, scale=scale, ranks=ranks, rows=plan.rows, tiles=plan.tiles)
+        _need_rows(y, "y"); _need_rows(x, "x"); _need(a, "a", x.dtype); _need(b, "b", x.dtype); _need(scale, "scale", torch.float32)
+        _need(plan.rows, "the plan's rows", torch.int32); _need(plan.tiles, "the plan's tiles", torch.int32)
+        (T, N), K = y.shape, x.shape[1]
+        widths = (N,) if widths is None else tuple(int(n) for n in widths)
+        if a.dim() != 4 or b.dim() != 3 or a.shape[1] != len(widths) or a.shape[3] != K or tuple(b.shape) != (a.shape[0], N, a.shape[2]) or sum(widths) != N:
+            raise KernelError(f"adapters_add_: a {tuple(a.shape)}, b {tuple(b.shape)} and widths {widths} do not fit x {tuple(x.shape)} and y {tuple(y.shape)}")
+        S, P, R, _ = a.shape
+        if x.shape[0] != T or plan.tokens > T or scale.numel() != S:
+            raise KernelError(f"adapters_add_: y has {T} rows, x {x.shape[0]}, the plan {plan.tokens}; {scale.numel()} scales for {S} slots")
+        if ranks is not None:
+            _need(ranks, "ranks", torch.int32)
+            if ranks.numel() != S:
+                raise KernelError(f"adapters_add_: {ranks.numel()} ranks for {S} slots")
+        self._call("roost_adapters_add", _ptr(y), y.stride(0) if T > 1 else N, _ptr(x), x.stride(0) if T > 1 else K, _ptr(a), _ptr(b), _ptr(scale), _ptr(ranks),
+                   _ptr(plan.rows), _ptr(plan.tiles), plan.tiles.shape[0], plan.rows.numel(), T, S, P, (c_int * P)(*widths), R, K, dtype_code(x.dtype),
+                   dtype_code(y.dtype), _stream())
+        return y
 
     def rope_table(self, positions: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
         """(cos, sin) of positions[t] * inv_freq[i] as float32 [T, half, 2]: a step computes it once for all its layers."""
