@@ -1,11 +1,651 @@
 // out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k] for rows in 8 bits (e4m3) with a scale a row on either side, 32-bit sums, one rounding.
 // The weight's scale comes first: its size is known to be ordinary, so rows of the largest and the least numbers stay in range on the way to their own.
+//
+// Operands that TMA can read (16-byte rows and strides) go to the tensor cores (tcgen05.mma kind::f8f6f4 but for the first) in one of four forms:
+//   a handful of rows of q and a small w: mma.sync on registers (gemm_e4m3_rows_kernel);
+//   few rows of q: 128 rows of w are the tile's rows and the rows of q its columns, k is split over a cluster (gemm_e4m3_split_kernel);
+//   more: persistent CTAs, one a processor, on tiles of 128 x 64, 128 or 256 (gemm_e4m3_tile_kernel);
+//   many: pairs of CTAs on tiles of 256 x 256 (gemm_e4m3_pair_kernel).
+// A block of k is 128 numbers, a row of the 128-byte swizzle. Every wait on a barrier has a limit, after which the kernel records a code (read back
+// with those of the bfloat16 products), lets its copies land, frees its tensor memory and returns.
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace roost {
 
+int* gemm_tcgen05_error_address();   // the error word of all tcgen05 products
+
+namespace {
+
+constexpr int kBlockK = 128;         // numbers (bytes) of a row in a stage
+
+// Instruction descriptor of kind::f8f6f4: D float32, A and B e4m3 (code 0), both K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+__device__ __forceinline__ void mma_e4m3(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a_desc),
+               "l"(b_desc), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d), "l"(a_desc),
+               "l"(b_desc), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  const uint16_t mask = 3;  // the barrier at this offset in both CTAs of the pair
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar), "h"(mask) : "memory");
+}
+// The load whose bytes count on a barrier of either CTA of the pair.
+__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c_inner, int c_outer) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c_inner), "r"(c_outer)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t rank_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t remote_address(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float load_remote(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void arrive_remote(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
+}
+// Every thread of the cluster that has not exited arrives and waits; the threads of a warp need not come together.
+__device__ __forceinline__ void sync_cluster() { asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(slot), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t base, uint32_t cols) {
+  tcgen05_fence_after();
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(cols) : "memory");
+}
+// After a wait was given up: time for copies in flight to land before shared memory is released.
+__device__ __forceinline__ void let_copies_land(volatile int* abortp) {
+  if (*abortp) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000LL) __nanosleep(256);
+  }
+}
+
+// 32 rows (a warp's lanes of tensor memory) of BN columns of an accumulator, scaled, to memory. 128 bytes of every row at a time go through a piece of
+// shared memory (4 KB a warp, 16-byte pieces swizzled by their row), so that eight lanes write a row's 128 bytes together: a store of 16 bytes of
+// 32 rows at once takes 32 turns where this takes 4, and the last tile's stores are not hidden by another tile.
+constexpr uint32_t kStoreBytes = 4 * 32 * 128;
+template <typename TOut, int N>
+__device__ __forceinline__ void put_piece(uint32_t buf, int row, int piece, const float (&o)[N]) {
+  uint32_t u[4];
+  if constexpr (sizeof(TOut) == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(o[2 * j], o[2 * j + 1]);
+      u[j] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = __float_as_uint(o[j]);
+  }
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(buf + row * 128 + ((piece ^ (row & 7)) << 4)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+}
+template <typename TOut, int BN>
+__device__ __forceinline__ void store_rows(TOut* out, int64_t ldo, uint32_t taddr, int row0, int n0, int M, int N, const float* q_scale, const float* w_scale,
+                                           uint32_t buf) {
+  constexpr int kVec = 16 / sizeof(TOut), kCols = 8 * kVec;   // columns of 128 bytes
+  const int lane = threadIdx.x & 31;
+  // rows that start on 16 bytes, else (and at the end of a row) single numbers, neighbours by neighbouring lanes
+  const bool whole = (ldo * (int64_t)sizeof(TOut)) % 16 == 0 && (uintptr_t)out % 16 == 0 && (uintptr_t)w_scale % 16 == 0;
+  const float rs = row0 + lane < M ? q_scale[row0 + lane] : 0.f;
+#pragma unroll 1
+  for (int c = 0; c < BN; c += kCols) {
+    const int col = n0 + c;
+    if (col >= N || row0 >= M) break;
+    uint32_t v[kCols];
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kCols / 32; ++i) tcgen05_ld_32x32b_x32_nowait(taddr + c + 32 * i, reinterpret_cast<uint32_t(&)[32]>(v[32 * i]));
+    tcgen05_wait_ld();
+    if (whole && col + kCols <= N) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        float o[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; j += 4) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(w_scale + col + p * kVec + j));
+          o[j] = f.x, o[j + 1] = f.y, o[j + 2] = f.z, o[j + 3] = f.w;
+        }
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) o[j] = __uint_as_float(v[p * kVec + j]) * o[j] * rs;
+        put_piece<TOut>(buf, lane, p, o);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + (lane >> 3), p = lane & 7;
+        uint4 u;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(buf + r * 128 + ((p ^ (r & 7)) << 4)) : "memory");
+        if (row0 + r < M) *reinterpret_cast<uint4*>(out + (int64_t)(row0 + r) * ldo + col + p * kVec) = u;
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        float o[kVec];
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) o[j] = __uint_as_float(v[p * kVec + j]) * __ldg(w_scale + min(col + p * kVec + j, N - 1)) * rs;
+        put_piece<TOut>(buf, lane, p, o);
+      }
+      __syncwarp();
+      const int rows = min(32, M - row0);
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r) {
+#pragma unroll
+        for (int h = 0; h < kCols; h += 32) {
+          const int e = h + lane;
+          const uint32_t at = buf + r * 128 + (((e / kVec) ^ (r & 7)) << 4) + (e % kVec) * (uint32_t)sizeof(TOut);
+          TOut* to = out + (int64_t)(row0 + r) * ldo + col + e;
+          if constexpr (sizeof(TOut) == 2) {
+            unsigned short u;
+            asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(u) : "r"(at) : "memory");
+            if (col + e < N) *reinterpret_cast<unsigned short*>(to) = u;
+          } else {
+            float u;
+            asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(u) : "r"(at) : "memory");
+            if (col + e < N) *to = u;
+          }
+        }
+      }
+    }
+  }
+}
+
+// Columns of a row of the accumulator that are rows of the output: the warp's lanes are neighbours in memory.
+template <typename TOut, int COLS>
+__device__ __forceinline__ void store_transposed(TOut* dst, int64_t ldo, const uint32_t (&v)[COLS], float w_scale, const float* q_scale, int valid) {
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) {
+    if (i < valid) dst[i * ldo] = from_float<TOut>(__uint_as_float(v[i]) * w_scale * __ldg(q_scale + i));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ a handful of rows
+// Latency is all there is to a product of up to 8 rows of q with a small w: a block takes 16 rows of w, its eight warps the blocks of 64 of k in turn,
+// straight from memory into the registers of mma.sync (m16n8k32): no barrier or copy engine lies between the loads and the products, and the first
+// kRowsDeep blocks of w are on their way before the wait for the kernel that makes q. A lane takes 16 numbers of a row at once; which k a
+// register of the instruction calls its own does not matter as long as both operands agree. The warps' sums meet in shared memory.
+constexpr int kRowsDeep = 8;
+__device__ __forceinline__ void mma_e4m3_k32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+template <typename TOut>
+__global__ void __launch_bounds__(256, 2)
+    gemm_e4m3_rows_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ w, const float* __restrict__ q_scale, const float* __restrict__ w_scale,
+                          TOut* __restrict__ out, int M, int N, int K, int64_t ldq, int64_t ldw, int64_t ldo) {
+  __shared__ float part[8][8][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int n0 = blockIdx.x * 16, blocks = (K + 63) / 64;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const uint8_t* w0 = w + (int64_t)min(n0 + g, N - 1) * ldw + 16 * c;
+  const uint8_t* w1 = w + (int64_t)min(n0 + g + 8, N - 1) * ldw + 16 * c;
+  float acc[4] = {};
+  uint4 a[kRowsDeep][2];
+  auto fetch = [&](int b0) {
+#pragma unroll
+    for (int i = 0; i < kRowsDeep; ++i) {
+      const int k = (b0 + 8 * i) * 64;
+      const bool in = k + 16 * c < K;
+      a[i][0] = in ? load_stream(w0 + k) : zero;
+      a[i][1] = in ? load_stream(w1 + k) : zero;
+    }
+  };
+  pdl_launch_dependents();
+  fetch(warp);
+  pdl_wait();
+  for (int b0 = warp; b0 < blocks; b0 += 8 * kRowsDeep) {
+    if (b0 != warp) fetch(b0);
+#pragma unroll
+    for (int i = 0; i < kRowsDeep; ++i) {
+      const int k = (b0 + 8 * i) * 64 + 16 * c;
+      const uint4 b = g < M && k < K ? *reinterpret_cast<const uint4*>(q + (int64_t)g * ldq + k) : zero;
+      mma_e4m3_k32(acc, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
+      mma_e4m3_k32(acc, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
+    }
+  }
+  part[warp][2 * c][g] = acc[0];
+  part[warp][2 * c + 1][g] = acc[1];
+  part[warp][2 * c][g + 8] = acc[2];
+  part[warp][2 * c + 1][g + 8] = acc[3];
+  __syncthreads();
+  const int i = threadIdx.x, n = n0 + (i & 15), m = i >> 4;
+  if (m < M && n < N) {
+    float sum = part[0][m][i & 15];
+#pragma unroll
+    for (int v = 1; v < 8; ++v) sum += part[v][m][i & 15];
+    out[(int64_t)m * ldo + n] = from_float<TOut>(sum * w_scale[n] * q_scale[m]);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// The weight's bytes are the time, so all that it takes is on its way at once: a cluster of `split` CTAs takes 128 rows of w, CTA r the r-th part of k,
+// two or three CTAs a processor, and every CTA asks for all its stages of w before it waits for the kernel that makes q. CTA o adds up the o-th part
+// of the tile's rows: the others send their sums for it straight from tensor memory into its shared memory and arrive on a barrier there, so that
+// nothing is asked for across the cluster and waited for; it adds them in CTA order.
+constexpr int kSplitStages = 8;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;\n" ::: "memory"); }
+__device__ __forceinline__ void send_vec(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+template <int NTOK>
+struct SplitCfg {
+  static constexpr uint32_t kStageW = 128 * kBlockK, kStage = kStageW + NTOK * kBlockK;
+  static constexpr int kPitch = NTOK + 4;                        // floats of a row of sums
+  static constexpr uint32_t kSums = 128 * kPitch * 4;            // the sums of all CTAs for this CTA's share: 128 rows in all
+};
+template <typename TOut, int NTOK>
+__global__ void __launch_bounds__(192, 2)
+    gemm_e4m3_split_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_q, const float* __restrict__ q_scale,
+                           const float* __restrict__ w_scale, TOut* __restrict__ out, int M, int N, int K, int64_t ldo, int split, int stages, int* error) {
+  using Cfg = SplitCfg<NTOK>;
+  constexpr uint32_t kStageW = Cfg::kStageW, kStage = Cfg::kStage, kCols = NTOK < 32 ? 32 : NTOK;
+  constexpr int kPitch = Cfg::kPitch;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t smem_base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
+  const uint32_t sums_base = smem_base + stages * kStage;
+  const float* sums = reinterpret_cast<const float*>(smem_raw + (sums_base - (uint32_t)__cvta_generic_to_shared(smem_raw)));   // [CTA][row of its share][kPitch]
+  __shared__ __align__(8) uint64_t bars[2 * kSplitStages + 2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kSplitStages + s); };
+  const uint32_t acc_full = bar0 + 8u * (2 * kSplitStages), sums_full = acc_full + 8u;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x / split, r = blockIdx.x % split;
+  const int share = 128 / split;                                // rows of the tile that a CTA adds up
+  const int m0 = blockIdx.y * NTOK;
+  q_scale += m0;
+  out += (int64_t)m0 * ldo;
+  M = min(M - m0, NTOK);
+  const int kbs = (K + kBlockK - 1) / kBlockK;
+  const int kb0 = (int)((int64_t)kbs * r / split), kb1 = (int)((int64_t)kbs * (r + 1) / split);  // kbs >= split
+  int ahead = 0;
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tma_w);
+    prefetch_tensormap(&tma_q);
+    abort_flag = 0;
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(sums_full, split * max(1, share / 32));           // a warp that sends arrives
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    pdl_launch_dependents();
+    for (int kb = kb0; kb < kb1 && ahead < stages; ++kb, ++ahead) {
+      mbar_expect_tx(full(ahead), kStage);
+      tma_load_2d(smem_base + ahead * kStage, &tma_w, full(ahead), kb * kBlockK, t * 128);
+    }
+  }
+  if (split > 1) cluster_arrive();     // the wait is ahead of the first word sent: by then every CTA runs and has its barriers
+  pdl_wait();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ahead; ++i) tma_load_2d(smem_base + i * kStage + kStageW, &tma_q, full(i), (kb0 + i) * kBlockK, m0);
+  }
+  if (warp == 1) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), kCols);
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abortp = &abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = ahead % stages;
+      uint32_t phase = ahead == stages ? 1u : 0u;
+      for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+        if (!mbar_wait_limited(empty(stage), phase ^ 1u, abortp, 1, error)) break;
+        const uint32_t sw = smem_base + stage * kStage;
+        mbar_expect_tx(full(stage), kStage);
+        tma_load_2d(sw, &tma_w, full(stage), kb * kBlockK, t * 128);
+        tma_load_2d(sw + kStageW, &tma_q, full(stage), kb * kBlockK, m0);
+        if (++stage == stages) stage = 0, phase ^= 1u;
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(128, NTOK);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = mbar_wait_limited(full(stage), phase, abortp, 3, error))) break;
+        tcgen05_fence_after();
+        const uint64_t a_desc = umma_desc_k_major_sw128(smem_base + stage * kStage);
+        const uint64_t b_desc = umma_desc_k_major_sw128(smem_base + stage * kStage + kStageW);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)   // 32 numbers, 32 bytes: two 16-byte units of the address field
+          mma_e4m3(tmem, a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+        tcgen05_commit(empty(stage));
+        if (++stage == stages) stage = 0, phase ^= 1u;
+      }
+      if (ok) tcgen05_commit(acc_full);
+    }
+  }
+  __syncwarp();
+  // every thread of the cluster comes here, whatever its waits returned
+  if (split > 1) cluster_wait();
+  if (warp >= 2) {
+    const bool ok = mbar_wait_limited(acc_full, 0u, abortp, 4, error);
+    // a lane of tensor memory is a row of w, a column a row of q
+    const int nl = (warp & 3) * 32 + lane, n = t * 128 + nl;
+    const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float ws = split == 1 && n < N ? w_scale[n] : 0.f;
+    const int owner = nl / share;
+    const uint32_t to = split > 1 ? remote_address(sums_base + (uint32_t)((r * share + nl % share) * kPitch) * 4u, owner) : 0u;
+    tcgen05_fence_after();
+#pragma unroll
+    for (int cb = 0; cb < NTOK; cb += 16) {
+      if (cb < M && ok) {
+        uint32_t v[16];
+        __syncwarp();
+        tcgen05_ld_32x32b_x16(taddr + cb, v);
+        if (split > 1) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            if (cb + i < M) send_vec(to + (uint32_t)(cb + i) * 4u, v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+        } else if (n < N) {
+          store_transposed<TOut>(out + (int64_t)cb * ldo + n, ldo, v, ws, q_scale + cb, M - cb);
+        }
+      }
+    }
+    tcgen05_fence_before();
+    if (split > 1) {
+      asm volatile("fence.acq_rel.cluster;\n" ::: "memory");
+      __syncwarp();
+      if (lane % share == 0) arrive_remote(remote_address(sums_full, owner));
+    }
+  }
+  if (split > 1) {
+    cluster_arrive();    // this CTA has sent all it has
+    if (warp >= 2) {
+      mbar_wait_limited<true>(sums_full, 0u, abortp, 5, error);
+      const int etid = threadIdx.x - 64, quads = (M + 3) / 4;
+      for (int i = etid; i < share * quads; i += 128) {
+        const int row = i % share, m = i / share * 4, n = t * 128 + r * share + row;
+        float4 part[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c < split) part[c] = *reinterpret_cast<const float4*>(sums + (c * share + row) * kPitch + m);
+        }
+        float4 sum = part[0];
+#pragma unroll
+        for (int c = 1; c < 8; ++c) {
+          if (c < split) sum.x += part[c].x, sum.y += part[c].y, sum.z += part[c].z, sum.w += part[c].w;
+        }
+        if (n < N) {
+          const float f = w_scale[n], o[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (m + j < M) out[(int64_t)(m + j) * ldo + n] = from_float<TOut>(o[j] * f * q_scale[m + j]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_wait();      // nobody leaves before all that is sent to it has come
+  }
+  let_copies_land(abortp);
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_free(tmem, kCols);
+}
+
+// ------------------------------------------------------------------------------------------------ more rows
+// One CTA a processor walks tiles of 128 x BN (m fastest, so that neighbours share a tile of w): warp 0 loads, warp 1 multiplies into one of two
+// accumulators, warps 2 to 5 scale and store the other one.
+constexpr int tile_stages(int bn) { return bn == 256 ? 4 : (bn == 128 ? 6 : 8); }
+template <typename TOut, int BN>
+__global__ void __launch_bounds__(192, 1)
+    gemm_e4m3_tile_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_w, const float* __restrict__ q_scale,
+                          const float* __restrict__ w_scale, TOut* __restrict__ out, int M, int N, int K, int64_t ldo, int* error) {
+  constexpr int kStages = tile_stages(BN);
+  constexpr uint32_t kStageA = 128 * kBlockK, kStage = kStageA + BN * kBlockK, kCols = 2 * BN;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t smem_base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto acc_full = [&](int a) { return bar0 + 8u * (2 * kStages + a); };
+  auto acc_empty = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    prefetch_tensormap(&tma_q);
+    prefetch_tensormap(&tma_w);
+  }
+  if (warp == 1) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), kCols);
+  tcgen05_fence_before();
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abortp = &abort_flag;
+  const int m_tiles = (M + 127) / 128, n_tiles = (N + BN - 1) / BN, kbs = (K + kBlockK - 1) / kBlockK, tiles = m_tiles * n_tiles;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const int m0 = (t % m_tiles) * 128, n0 = (t / m_tiles) * BN;
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!(ok = mbar_wait_limited(empty(stage), phase ^ 1u, abortp, 1, error))) break;
+          const uint32_t sa = smem_base + stage * kStage;
+          mbar_expect_tx(full(stage), kStage);
+          tma_load_2d(sa, &tma_q, full(stage), kb * kBlockK, m0);
+          tma_load_2d(sa + kStageA, &tma_w, full(stage), kb * kBlockK, n0);
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(128, BN);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++it) {
+        const int acc = it & 1;
+        if (!(ok = mbar_wait_limited(acc_empty(acc), ((uint32_t)(it >> 1) & 1u) ^ 1u, abortp, 2, error))) break;
+        tcgen05_fence_after();
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!(ok = mbar_wait_limited(full(stage), phase, abortp, 3, error))) break;
+          tcgen05_fence_after();
+          const uint64_t a_desc = umma_desc_k_major_sw128(smem_base + stage * kStage);
+          const uint64_t b_desc = umma_desc_k_major_sw128(smem_base + stage * kStage + kStageA);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_e4m3(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          tcgen05_commit(empty(stage));
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+        if (ok) tcgen05_commit(acc_full(acc));
+      }
+    }
+  } else {
+    const int lanes = (warp & 3) * 32;
+    int it = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++it) {
+      const int acc = it & 1, row = (t % m_tiles) * 128 + lanes, n0 = (t / m_tiles) * BN;
+      if (!mbar_wait_limited(acc_full(acc), (uint32_t)(it >> 1) & 1u, abortp, 4, error)) break;
+      tcgen05_fence_after();
+      store_rows<TOut, BN>(out, ldo, tmem + ((uint32_t)lanes << 16) + (uint32_t)(acc * BN), row, n0, M, N, q_scale, w_scale, smem_base + kStages * kStage + lanes * 128);
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty(acc));
+    }
+  }
+  __syncwarp();
+  let_copies_land(abortp);
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_free(tmem, kCols);
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+// Two CTAs on one 256 x 256 tile (tcgen05.mma.cta_group::2): each stages its own 128 rows of q and 128 rows of w, half as much a product as one CTA
+// alone would. The even CTA issues every product; both CTAs' loads count on its barrier, its commit releases the stage in both, and each CTA's
+// warps 2 to 5 store their own 128 rows. No load is multicast.
+constexpr int kPairStages = 6;
+template <typename TOut>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+    gemm_e4m3_pair_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_w, const float* __restrict__ q_scale,
+                          const float* __restrict__ w_scale, TOut* __restrict__ out, int M, int N, int K, int64_t ldo, int* error) {
+  constexpr int kStages = kPairStages, BN = 256;
+  constexpr uint32_t kStageA = 128 * kBlockK, kStage = 2 * kStageA, kCols = 2 * BN;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t smem_base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
+  auto full = [&](int s) { return bar0 + 8u * s; };
+  auto empty = [&](int s) { return bar0 + 8u * (kStages + s); };
+  auto acc_full = [&](int a) { return bar0 + 8u * (2 * kStages + a); };
+  auto acc_empty = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = rank_in_cluster();
+  if (threadIdx.x == 0) {
+    abort_flag = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(acc_full(a), 1);
+      mbar_init(acc_empty(a), 8);  // four warps in each CTA of the pair
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    prefetch_tensormap(&tma_q);
+    prefetch_tensormap(&tma_w);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_slot)), "r"(kCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+  tcgen05_fence_before();
+  pdl_launch_dependents();
+  pdl_wait();
+  __syncthreads();
+  sync_cluster();  // both CTAs' barriers exist before anyone arrives on the other's
+  tcgen05_fence_after();
+  const uint32_t tmem = tmem_slot;
+  volatile int* abortp = &abort_flag;
+  const int m_tiles = (M + 255) / 256, n_tiles = (N + 255) / 256, kbs = (K + kBlockK - 1) / kBlockK, tiles = m_tiles * n_tiles;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t even_full = remote_address(full(0), 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int m0 = (t % m_tiles) * 256 + (int)rank * 128, n0 = (t / m_tiles) * 256 + (int)rank * 128;
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!(ok = mbar_wait_limited(empty(stage), phase ^ 1u, abortp, 1, error))) break;
+          const uint32_t sa = smem_base + stage * kStage;
+          if (rank == 0) mbar_expect_tx(full(stage), 2 * kStage);
+          load_2d_pair(sa, &tma_q, even_full + 8u * stage, kb * kBlockK, m0);
+          load_2d_pair(sa + kStageA, &tma_w, even_full + 8u * stage, kb * kBlockK, n0);
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(256, BN);
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, ++it) {
+        const int acc = it & 1;
+        if (!(ok = mbar_wait_limited<true>(acc_empty(acc), ((uint32_t)(it >> 1) & 1u) ^ 1u, abortp, 2, error))) break;
+        tcgen05_fence_after();
+        for (int kb = 0; kb < kbs; ++kb) {
+          if (!(ok = mbar_wait_limited<true>(full(stage), phase, abortp, 3, error))) break;
+          tcgen05_fence_after();
+          const uint64_t a_desc = umma_desc_k_major_sw128(smem_base + stage * kStage);
+          const uint64_t b_desc = umma_desc_k_major_sw128(smem_base + stage * kStage + kStageA);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_e4m3_pair(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+          commit_pair(empty(stage));
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+        if (ok) commit_pair(acc_full(acc));
+      }
+    }
+  } else {
+    const int lanes = (warp & 3) * 32;
+    const uint32_t even_acc_empty[2] = {remote_address(acc_empty(0), 0), remote_address(acc_empty(1), 0)};
+    int it = 0;
+    for (int t = pair; t < tiles; t += pairs, ++it) {
+      const int acc = it & 1, row = (t % m_tiles) * 256 + (int)rank * 128 + lanes, n0 = (t / m_tiles) * 256;
+      if (!mbar_wait_limited(acc_full(acc), (uint32_t)(it >> 1) & 1u, abortp, 4, error)) break;
+      tcgen05_fence_after();
+      store_rows<TOut, 256>(out, ldo, tmem + ((uint32_t)lanes << 16) + (uint32_t)(acc * BN), row, n0, M, N, q_scale, w_scale, smem_base + kStages * kStage + lanes * 128);
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_remote(even_acc_empty[acc]);
+    }
+  }
+  __syncwarp();
+  let_copies_land(abortp);
+  tcgen05_fence_before();
+  __syncthreads();
+  sync_cluster();  // neither CTA frees shared or tensor memory the other may still be using
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kCols) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ any size
 __device__ __forceinline__ float e4m3_float(uint8_t v) {
   const __half_raw h = __nv_cvt_fp8_to_halfraw(v, __NV_E4M3);
   return __half2float(*reinterpret_cast<const __half*>(&h));
@@ -52,6 +692,161 @@ __global__ void __launch_bounds__(256) gemm_e4m3_any_kernel(const uint8_t* __res
   }
 }
 
+// ------------------------------------------------------------------------------------------------ host side
+// A matrix of rows of k bytes, ld apart, in boxes of box_rows x 128.
+int make_map(CUtensorMap* map, const void* base, int rows, int k, int64_t ld, int box_rows) {
+  EncodeTiledFn enc = encode_tiled();
+  if (!enc) return fail(ROOST_ERR_CUDA, "gemm_e4m3: the driver does not export cuTensorMapEncodeTiled");
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows};
+  const cuuint32_t elem[2] = {1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ROOST_ERR_CUDA, "gemm_e4m3: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return ROOST_OK;
+}
+
+// Shared memory beyond 48 KB is allowed a kernel once a device.
+template <typename Kernel>
+void allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+struct Operands {
+  const void *q, *w;
+  const float *q_scale, *w_scale;
+  void* out;
+  int m, n, k;
+  int64_t ldq, ldw, ldo;
+  int* error;
+  cudaStream_t stream;
+};
+
+// The few-row form: `split` CTAs a tile, as many (up to 8) as leave a processor one CTA, and two blocks of k for each: a processor's second CTA waits for
+// the same tensor cores, and the sums of a cluster cost more than it brings (8 x 4,096 x 4,096: split 4 6.6 us, 8 8.2, 2 8.3; 8 x 12,288 x 4,096:
+// 1 12.7, 2 14.1; 8 x 24,576 x 4,096: 1 19.6, 2 22.9).
+int split_of(int64_t tiles, int k) {
+  const int kbs = (k + kBlockK - 1) / kBlockK;
+  int split = 8;
+  while (split > 1 && (tiles * split > processors() || split > kbs / 2)) split /= 2;
+  return split;
+}
+
+template <typename TOut, int NTOK>
+int launch_split(const Operands& o) {
+  static std::atomic<uint64_t> done{0};
+  using Cfg = SplitCfg<NTOK>;
+  const int tiles = (o.n + 127) / 128, chunks = (o.m + NTOK - 1) / NTOK, split = split_of((int64_t)tiles * chunks, o.k);
+  const int kbs = (o.k + kBlockK - 1) / kBlockK;
+  // Six stages, four for a short part of k (8 x 4,096 x 4,096: 6.6 us, 7.2 with six); where a processor has two CTAs, as many as let both in.
+  const size_t sums = split > 1 ? Cfg::kSums : 0, room = ((int64_t)tiles * chunks * split > processors() ? 112 : 224) * 1024 - 1024 - sums;
+  int stages = kbs / split <= 8 ? 4 : 6;
+  while (stages > 2 && stages * (size_t)Cfg::kStage > room) --stages;
+  const size_t smem = stages * (size_t)Cfg::kStage + sums + 1024;
+  CUtensorMap mw, mq;
+  int rc = make_map(&mw, o.w, o.n, o.k, o.ldw, 128);
+  if (rc == ROOST_OK) rc = make_map(&mq, o.q, o.m, o.k, o.ldq, NTOK);
+  if (rc != ROOST_OK) return rc;
+  auto kernel = gemm_e4m3_split_kernel<TOut, NTOK>;
+  allow_smem(kernel, 224 * 1024, done);
+  launch_kernel_cluster(kernel, dim3(tiles * split, chunks), dim3(192), smem, o.stream, split, mw, mq, o.q_scale, o.w_scale, (TOut*)o.out, o.m, o.n, o.k, o.ldo,
+                        split, stages, o.error);
+  return check_launch("gemm_e4m3 (few rows)");
+}
+
+template <typename TOut, int BN>
+int launch_tile(const Operands& o) {
+  static std::atomic<uint64_t> done{0};
+  const size_t smem = (size_t)tile_stages(BN) * (128 + BN) * kBlockK + kStoreBytes + 1024;
+  CUtensorMap mq, mw;
+  int rc = make_map(&mq, o.q, o.m, o.k, o.ldq, 128);
+  if (rc == ROOST_OK) rc = make_map(&mw, o.w, o.n, o.k, o.ldw, BN);
+  if (rc != ROOST_OK) return rc;
+  auto kernel = gemm_e4m3_tile_kernel<TOut, BN>;
+  allow_smem(kernel, smem, done);
+  const int64_t tiles = (int64_t)((o.m + 127) / 128) * ((o.n + BN - 1) / BN);
+  const int grid = (int)(tiles < processors() ? tiles : processors());
+  launch_kernel(kernel, dim3(grid), dim3(192), smem, o.stream, mq, mw, o.q_scale, o.w_scale, (TOut*)o.out, o.m, o.n, o.k, o.ldo, o.error);
+  return check_launch("gemm_e4m3 (tiles)");
+}
+
+template <typename TOut>
+int launch_pair(const Operands& o) {
+  static std::atomic<uint64_t> done{0};
+  const size_t smem = (size_t)kPairStages * 256 * kBlockK + kStoreBytes + 1024;
+  CUtensorMap mq, mw;
+  int rc = make_map(&mq, o.q, o.m, o.k, o.ldq, 128);
+  if (rc == ROOST_OK) rc = make_map(&mw, o.w, o.n, o.k, o.ldw, 128);
+  if (rc != ROOST_OK) return rc;
+  auto kernel = gemm_e4m3_pair_kernel<TOut>;
+  allow_smem(kernel, smem, done);
+  const int64_t tiles = (int64_t)((o.m + 255) / 256) * ((o.n + 255) / 256);
+  const int pairs = (int)(tiles < processors() / 2 ? tiles : processors() / 2);
+  launch_kernel(kernel, dim3(2 * pairs), dim3(192), smem, o.stream, mq, mw, o.q_scale, o.w_scale, (TOut*)o.out, o.m, o.n, o.k, o.ldo, o.error);
+  return check_launch("gemm_e4m3 (pairs)");
+}
+
+template <typename TOut>
+int launch_rows(const Operands& o) {
+  launch_kernel(gemm_e4m3_rows_kernel<TOut>, dim3((o.n + 15) / 16), dim3(256), 0, o.stream, (const uint8_t*)o.q, (const uint8_t*)o.w, o.q_scale, o.w_scale,
+                (TOut*)o.out, o.m, o.n, o.k, o.ldq, o.ldw, o.ldo);
+  return check_launch("gemm_e4m3 (a handful of rows)");
+}
+
+template <typename TOut>
+int launch_any(const Operands& o) {
+  const int rows = (o.m + kAnyTile - 1) / kAnyTile;
+  const dim3 grid((o.n + kAnyTile - 1) / kAnyTile, rows < 65535 ? rows : 65535);
+  launch_kernel(gemm_e4m3_any_kernel<TOut>, grid, dim3(256), 0, o.stream, (const uint8_t*)o.q, o.q_scale, (const uint8_t*)o.w, o.w_scale, (TOut*)o.out, o.m, o.n, o.k,
+                o.ldq, o.ldw, o.ldo);
+  return check_launch("gemm_e4m3 (any size)");
+}
+
+// The form with the least time by a count of its steps: rounds of tiles over the processors, a block of k each, and what a launch takes beside. A block of k
+// takes as long for 128 columns as for 64 (a product of 128 x 32 from shared memory takes 128 cycles up to there), 0.41 us for 256 and 0.37 for a
+// pair's 256 x 256, measured over 4,096 x 4,096 x 12,288 (385, 193, 155 and 143 us); beside it 512 rows x 4,096 x 4,096 took 3.7, 4.2, 4.1 and 4.4 us more.
+enum Form { kTile64, kTile128, kTile256, kPair, kSplit };
+Form form_of(int m, int n, int k) {
+  const int64_t sms = processors(), kbs = (k + kBlockK - 1) / kBlockK;
+  const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const float cost[5] = {up(up(m, 128) * up(n, 64), sms) * kbs * 0.272f + 3.7f, up(up(m, 128) * up(n, 128), sms) * kbs * 0.287f + 4.2f,
+                         up(up(m, 128) * up(n, 256), sms) * kbs * 0.405f + 4.1f, up(up(m, 256) * up(n, 256), sms / 2) * kbs * 0.373f + 4.4f,
+                         up(up(m, 128) * up(n, 128) * split_of(up(m, 128) * up(n, 128), k), sms) * up(kbs, split_of(up(m, 128) * up(n, 128), k)) * 0.3f + 8.0f};
+  int best = 0;
+  for (int i = 1; i < 5; ++i) {
+    if (cost[i] < cost[best]) best = i;
+  }
+  return (Form)best;
+}
+
+template <typename TOut>
+int launch_gemm(const Operands& o) {
+  const bool tma = o.k % 16 == 0 && o.ldq % 16 == 0 && o.ldw % 16 == 0 && (uintptr_t)o.q % 16 == 0 && (uintptr_t)o.w % 16 == 0;
+  if (!tma) return launch_any<TOut>(o);
+  // A handful of rows whose strips of w all run at once, two blocks a processor; one, where a warp asks more than once for its part of k. Against the
+  // split form: 8 x 4,096 x 4,096 5.7 us, 7.0; 8 x 1,024 x 4,096 4.3, 5.0; 8 x 2,000 x 16,000 14.5, 17.1; but 8 x 4,096 x 12,288 14.1, 12.1 and
+  // 8 x 24,576 x 4,096 25.8, 19.3.
+  const int strips = (o.n + 15) / 16;
+  if (o.m <= 8 && (strips <= processors() || (strips <= 2 * processors() && o.k <= 64 * 8 * kRowsDeep))) return launch_rows<TOut>(o);
+  if (o.m <= 16) return launch_split<TOut, 16>(o);
+  if (o.m <= 32) return launch_split<TOut, 32>(o);
+  if (o.m <= 64) return launch_split<TOut, 64>(o);
+  switch (form_of(o.m, o.n, o.k)) {
+    case kTile64: return launch_tile<TOut, 64>(o);
+    case kTile128: return launch_tile<TOut, 128>(o);
+    case kTile256: return launch_tile<TOut, 256>(o);
+    case kPair: return launch_pair<TOut>(o);
+    default: return launch_split<TOut, 128>(o);
+  }
+}
+
+}  // namespace
 }  // namespace roost
 
 using namespace roost;
@@ -62,12 +857,10 @@ extern "C" int roost_gemm_e4m3(const void* q, const float* q_scale, const void* 
   ROOST_REQUIRE(ldq >= k && ldw >= k && ldo >= n, "gemm_e4m3: a leading dimension is smaller than its row");
   if (m == 0) return ROOST_OK;
   ROOST_REQUIRE(q && q_scale && w && w_scale && out, "gemm_e4m3: a pointer is null");
-  const int rows = (m + kAnyTile - 1) / kAnyTile;
-  const dim3 grid((n + kAnyTile - 1) / kAnyTile, rows < 65535 ? rows : 65535);
-  ROOST_DISPATCH_DTYPE(out_dtype, TOut,
-                       launch_kernel(gemm_e4m3_any_kernel<TOut>, grid, dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)q, q_scale, (const uint8_t*)w, w_scale,
-                                     (TOut*)out, m, n, k, ldq, ldw, ldo));
-  return check_launch("gemm_e4m3");
+  if (n > 2147483647 - 256 || m > 2147483647 - 256) return fail(ROOST_ERR_UNSUPPORTED, "gemm_e4m3: more rows than a tile's index holds");
+  Operands o{q, w, q_scale, w_scale, out, m, n, k, ldq, ldw, ldo, gemm_tcgen05_error_address(), (cudaStream_t)stream};
+  if (!o.error) return fail(ROOST_ERR_CUDA, "gemm_e4m3: the error word has no device address");
+  ROOST_DISPATCH_DTYPE(out_dtype, TOut, return launch_gemm<TOut>(o));
 }
 
 ROOST_TRACE_TU(gemm_e4m3)
