@@ -244,8 +244,9 @@ _SIGNATURES = {
     "roost_silu_mul_e4m3": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "roost_rms_norm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p],
     "roost_gemm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
-    "roost_adapters_add": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
-                           c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "roost_adapters_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
+    "roost_adapters_add": [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                           c_int, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "roost_argmax": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p],
     "roost_argmax_split": [c_void_p, c_int64, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "roost_sample": [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -281,14 +282,17 @@ class AdapterPlan:
     rows: torch.Tensor
     tiles: torch.Tensor
     tokens: int
+    tile_rows: int = 64      # tokens of a tile at most
 
 
-ADAPTER_TILE_ROWS = 64   # tokens of a tile of an adapter plan at most
+ADAPTER_TILE_ROWS = 64       # tokens of a tile of an adapter plan at most
+ADAPTER_FEW_ROWS = 16        # ... where tiles of this many still leave processors without work
+ADAPTER_FEW_TILES = 37
 
 
 def adapter_lists(row_counts: list, row_slots: list) -> tuple:
-    """(rows, tiles) of an ``AdapterPlan`` as int32 numpy arrays, for a step whose i-th request brings ``row_counts[i]`` tokens and uses the adapter
-    in slot ``row_slots[i]`` (negative: none)."""
+    """(rows, tiles, tile_rows) of an ``AdapterPlan`` as int32 numpy arrays, for a step whose i-th request brings ``row_counts[i]`` tokens and uses the
+    adapter in slot ``row_slots[i]`` (negative: none)."""
     if len(row_counts) != len(row_slots):
         raise KernelError(f"adapter_plan: {len(row_counts)} requests, {len(row_slots)} adapters")
     counts, slots = np.asarray(row_counts, np.int64), np.asarray(row_slots, np.int64)
@@ -299,8 +303,16 @@ def adapter_lists(row_counts: list, row_slots: list) -> tuple:
     rows = order[np.searchsorted(of[order], 0):]                    # tokens without an adapter are left out
     used, first = np.unique(of[rows], return_index=True)
     ends = np.append(first[1:], rows.size)
-    tiles = [(s, at, min(at + ADAPTER_TILE_ROWS, end)) for s, lo, end in zip(used, first, ends) for at in range(lo, end, ADAPTER_TILE_ROWS)]
-    return rows.astype(np.int32), np.asarray(tiles, np.int32).reshape(-1, 3)
+
+    def cut(most):
+        return [(s, at, min(at + most, end)) for s, lo, end in zip(used, first, ends) for at in range(lo, end, most)]
+
+    tile_rows = ADAPTER_FEW_ROWS
+    tiles = cut(tile_rows)
+    if len(tiles) > ADAPTER_FEW_TILES and max(end - at for _, at, end in tiles) == tile_rows:
+        tile_rows = ADAPTER_TILE_ROWS
+        tiles = cut(tile_rows)
+    return rows.astype(np.int32), np.asarray(tiles, np.int32).reshape(-1, 3), tile_rows
 
 
 MOE_TCGEN05_MIN_ROWS = 1024  # sorted rows from which a bfloat16 step runs the experts' products on tcgen05
@@ -319,7 +331,7 @@ class KernelLibrary:
         for name, args in _SIGNATURES.items():
             fn = getattr(self._lib, name)
             fn.argtypes = args
-            fn.restype = c_int
+            fn.restype = c_int64 if name.endswith("_bytes") else c_int
         self.decode_chunk = 512  # keys per work item of the split decode attention (see decode_chunk_for)
         self.decode_cluster = True  # split rows merged by thread-block clusters where they fit (see decode_cluster_for)
         self._decode_ctas = 0
@@ -497,9 +509,9 @@ class KernelLibrary:
     def adapter_plan(self, row_counts: list, row_slots: list, device=None) -> AdapterPlan:
         """The lists by which ``adapters_add_`` deals a step's tokens out, for all the step's layers: request i brings ``row_counts[i]`` tokens, one
         request after the other, and uses the adapter in slot ``row_slots[i]`` (negative: none)."""
-        rows, tiles = adapter_lists(row_counts, row_slots)
+        rows, tiles, tile_rows = adapter_lists(row_counts, row_slots)
         both = torch.from_numpy(np.concatenate([tiles.reshape(-1), rows])).to(device if device is not None else "cuda")
-        return AdapterPlan(rows=both[tiles.size:], tiles=both[:tiles.size].view(-1, 3), tokens=int(sum(row_counts)))
+        return AdapterPlan(rows=both[tiles.size:], tiles=both[:tiles.size].view(-1, 3), tokens=int(sum(row_counts)), tile_rows=tile_rows)
 
     def adapters_add_(self, y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, plan: AdapterPlan,
                       widths: tuple | None = None, ranks: torch.Tensor | None = None) -> torch.Tensor:
@@ -521,9 +533,12 @@ class KernelLibrary:
             _need(ranks, "ranks", torch.int32)
             if ranks.numel() != S:
                 raise KernelError(f"adapters_add_: {ranks.numel()} ranks for {S} slots")
-        self._call("roost_adapters_add", _ptr(y), y.stride(0) if T > 1 else N, _ptr(x), x.stride(0) if T > 1 else K, _ptr(a), _ptr(b), _ptr(scale), _ptr(ranks),
-                   _ptr(plan.rows), _ptr(plan.tiles), plan.tiles.shape[0], plan.rows.numel(), T, S, P, (c_int * P)(*widths), R, K, dtype_code(x.dtype),
-                   dtype_code(y.dtype), _stream())
+        codes, listed = (dtype_code(x.dtype), dtype_code(y.dtype)), plan.rows.numel()
+        need = self._lib.roost_adapters_workspace_bytes(listed, P, R, *codes)
+        h = torch.empty(need, dtype=torch.uint8, device=y.device) if need else None
+        self._call("roost_adapters_add", _ptr(y), y.stride(0) if T > 1 else N, _ptr(x), x.stride(0) if T > 1 else K, _ptr(a), _ptr(b), _ptr(h), _ptr(scale),
+                   _ptr(ranks), _ptr(plan.rows), _ptr(plan.tiles), plan.tiles.shape[0], plan.tile_rows, listed, T, S, P, (c_int * P)(*widths), R, K, *codes,
+                   _stream(), launches=2 if need else 1)
         return y
 
     def rope_table(self, positions: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
