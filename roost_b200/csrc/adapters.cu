@@ -147,6 +147,12 @@ __device__ __forceinline__ void adapter_split(float v, __nv_bfloat16 (&o)[SPLIT]
   }
 }
 __device__ __forceinline__ uint4 adapter_load16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+// The same from what the kernel in front wrote.
+__device__ __forceinline__ uint4 adapter_load16_new(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 // The first n (at most 8) of eight bfloat16 numbers, zeros behind them.
 __device__ __forceinline__ uint4 adapter_first(uint4 v, int n) {
   if (n >= 8) return v;
@@ -173,109 +179,127 @@ __device__ __forceinline__ int adapter_row(const int32_t* rows, int at, int toke
   return r >= 0 && r < tokens ? r : -1;
 }
 
-// MT tiles of 16 tokens; G tiles of 8 rows of a for a warp at a time; h [SPLIT][listed][parts * r32] with r32 = R rounded up to 32.
-template <int SPLIT, int MT, int G, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, CTAS) __cluster_dims__(kAdapterCluster, 1, 1)
+// A cluster of `ctas` takes a tile of up to MT * 16 tokens, CTA v the v-th part of k. Sixteen warps, one CTA a processor: warps side by side on groups of G
+// tiles of 8 rows of a, and on k with what is left of them; a warp's loads of a block of 32 of k (2 MT of x, G of a) are on their way together, a's for
+// the next block as soon as the products have read this one's. h [SPLIT][listed][parts * r32], r32 = R rounded up to 32.
+constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
+template <int SPLIT, int MT, int G>
+__global__ void __launch_bounds__(kDownThreads, 1)
     adapters_down_kernel(__nv_bfloat16* __restrict__ h_out, const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ a,
                          const float* __restrict__ scales, const int32_t* __restrict__ ranks, const int32_t* __restrict__ rows, const int32_t* __restrict__ tiles,
-                         int tokens, int listed, int slots, int parts, int R, int K) {
-  extern __shared__ __align__(16) float h[];     // [warps along k][tokens of the tile][parts * rank, in whole tiles of 8]
-  constexpr int kWarps = THREADS / 32;
+                         int tokens, int listed, int slots, int parts, int R, int K, int ctas) {
+  extern __shared__ __align__(16) float h[];     // [warps along k][tokens of the tile][parts * rank, in whole tiles of 8, and what fills the pitch]
   pdl_launch_dependents();
-  const int tile = blockIdx.x / kAdapterCluster, cta = (int)adapter_cluster_rank();
-  const AdapterTile at = adapter_tile(tiles, tile, ranks, MT * 16, listed, slots, R);
+  const int cta = (int)adapter_cluster_rank();
+  const AdapterTile at = adapter_tile(tiles, blockIdx.x / ctas, ranks, MT * 16, listed, slots, R);
+  if (at.rank == 0) {    // the whole cluster
+    pdl_wait();
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
   const int nt = (at.rank + 7) / 8, rp = 8 * nt, wide = parts * rp, n_tiles = parts * nt;
+  const int pitch = wide + ((40 - wide % 32) & 31);     // floats of a token's sums: 8 beyond a multiple of 32, so that a warp's stores meet all banks
+  const float factor = scales[at.slot];
+  // Rows that do not exist (tokens behind the tile's, ranks behind the slot's) are read from ones that do: each makes numbers of its own row of h only,
+  // and those are not used.
   const __nv_bfloat16* xr[2 * MT];
 #pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) {
-    const int r = g + 8 * i < at.rows ? adapter_row(rows, at.first + g + 8 * i, tokens) : -1;
-    xr[i] = r >= 0 ? x + (int64_t)r * ldx + 8 * c : nullptr;
-  }
-  // warps side by side on the tiles of a as far as G each cover them, on k beyond that
-  int wn = 1;
-  while (wn < kWarps && wn * G < n_tiles) wn *= 2;
-  const int wk = kWarps / wn, my_n = warp % wn, my_k = warp / wn;
-  const int blocks = (K + 31) / 32, kb0 = (int)((int64_t)blocks * cta / kAdapterCluster) + my_k, kb1 = (int)((int64_t)blocks * (cta + 1) / kAdapterCluster);
+  for (int i = 0; i < 2 * MT; ++i) xr[i] = x + (int64_t)max(adapter_row(rows, at.first + min(g + 8 * i, at.rows - 1), tokens), 0) * ldx + 8 * c;
+  const int groups = min((n_tiles + G - 1) / G, kDownWarps), wk = kDownWarps / groups, my_k = warp / groups;
+  const int blocks = (K + 31) / 32, whole = K / 32;
+  const int kb0 = (int)((int64_t)blocks * cta / ctas) + my_k, kb1 = my_k < wk ? (int)((int64_t)blocks * (cta + 1) / ctas) : 0;
   a += (int64_t)at.slot * parts * R * K;
   bool waited = false;
-  for (int t0 = my_n * G; t0 < n_tiles; t0 += wn * G) {
+  for (int t0 = warp % groups * G; t0 < n_tiles; t0 += groups * G) {
     float acc[MT][G][4] = {};
     const __nv_bfloat16* ar[G];
 #pragma unroll
     for (int t = 0; t < G; ++t) {
-      const int p = (t0 + t) / nt, r = (t0 + t) % nt * 8 + g;
-      ar[t] = t0 + t < n_tiles && r < at.rank ? a + ((int64_t)p * R + r) * K + 8 * c : nullptr;
+      const int tt = min(t0 + t, n_tiles - 1), r = min(tt % nt * 8 + g, at.rank - 1);
+      ar[t] = a + ((int64_t)(tt / nt) * R + r) * K + 8 * c;
     }
-    uint4 av[G];
-    auto fetch = [&](int kb) {
-      const bool in = kb < kb1 && kb * 32 + 8 * c < K;
-#pragma unroll
-      for (int t = 0; t < G; ++t) av[t] = ar[t] && in ? adapter_load16(ar[t] + kb * 32) : zero;
-    };
-    fetch(kb0);
-    if (!waited) pdl_wait();
-    waited = true;
-    for (int kb = kb0; kb < kb1; kb += wk) {
-      uint4 xv[2 * MT], an[G];
-      const bool in = kb * 32 + 8 * c < K;
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) xv[i] = xr[i] && in ? adapter_load16(xr[i] + kb * 32) : zero;
-#pragma unroll
-      for (int t = 0; t < G; ++t) an[t] = av[t];
-      fetch(kb + wk);
+    uint4 xv[2 * MT], av[G];
+    auto multiply = [&]() {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const uint32_t lo[4] = {xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y}, hi[4] = {xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w};
 #pragma unroll
         for (int t = 0; t < G; ++t) {
-          mma_bf16(acc[m][t], lo, an[t].x, an[t].y);
-          mma_bf16(acc[m][t], hi, an[t].z, an[t].w);
+          mma_bf16(acc[m][t], lo, av[t].x, av[t].y);
+          mma_bf16(acc[m][t], hi, av[t].z, av[t].w);
         }
       }
+    };
+    auto fetch_a = [&](int kb) {
+      if (kb < min(kb1, whole)) {
+#pragma unroll
+        for (int t = 0; t < G; ++t) av[t] = adapter_load16(ar[t] + kb * 32);
+      }
+    };
+    fetch_a(kb0);
+    if (!waited) pdl_wait();
+    waited = true;
+    int kb = kb0;
+#pragma unroll 1
+    for (; kb < min(kb1, whole); kb += wk) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) xv[i] = adapter_load16(xr[i] + kb * 32);
+      multiply();
+      fetch_a(kb + wk);
     }
+    if (kb < kb1) {      // the last block where K is no multiple of 32: zeros behind its end in both
+      const bool in = kb * 32 + 8 * c < K;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int t = 0; t < G; ++t) {
-      if (t0 + t >= n_tiles) continue;
+      for (int t = 0; t < G; ++t) av[t] = in ? adapter_load16(ar[t] + kb * 32) : zero;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
+      for (int i = 0; i < 2 * MT; ++i) xv[i] = in ? adapter_load16(xr[i] + kb * 32) : zero;
+      multiply();
+    }
+    if (my_k < wk) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = m * 16 + g + 8 * e;
-          if (i < at.rows) *reinterpret_cast<float2*>(h + (my_k * at.rows + i) * wide + (t0 + t) * 8 + 2 * c) = make_float2(acc[m][t][2 * e], acc[m][t][2 * e + 1]);
+      for (int t = 0; t < G; ++t) {
+        if (t0 + t >= n_tiles) continue;
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int i = m * 16 + g + 8 * e;
+            if (i < at.rows) *reinterpret_cast<float2*>(h + (my_k * at.rows + i) * pitch + (t0 + t) * 8 + 2 * c) = make_float2(acc[m][t][2 * e], acc[m][t][2 * e + 1]);
+          }
         }
       }
     }
   }
   if (!waited) pdl_wait();
-  if (at.rank == 0) return;    // the whole cluster
-  const int count = at.rows * wide;
+  const int count = at.rows * pitch;
   if (wk > 1) {
     __syncthreads();
-    for (int e = threadIdx.x; e < count; e += THREADS) {
+    for (int e = threadIdx.x; e < count; e += kDownThreads) {
       float sum = h[e];
+#pragma unroll 4
       for (int v = 1; v < wk; ++v) sum += h[v * count + e];
       h[e] = sum;
     }
   }
   adapter_cluster_sync();
-  const float factor = scales[at.slot];
-  const int r32 = (R + 31) & ~31, used32 = (at.rank + 31) & ~31, line = parts * used32, all = at.rows * line;
-  uint32_t from[kAdapterCluster];
-#pragma unroll
-  for (int v = 0; v < kAdapterCluster; ++v) from[v] = adapter_remote((uint32_t)__cvta_generic_to_shared(h), v);
-  const int e1 = (int)((int64_t)all * (cta + 1) / kAdapterCluster);
-  for (int e = (int)((int64_t)all * cta / kAdapterCluster) + threadIdx.x; e < e1; e += THREADS) {
-    const int i = e / line, j = e % line, p = j / used32, r = j % used32;
+  // a warp 32 numbers of a token's part at a time, a CTA its share of them
+  const int r32 = (R + 31) & ~31, nb = (at.rank + 31) / 32, pieces = at.rows * parts * nb;
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(h);
+  const int q1 = (int)((int64_t)pieces * (cta + 1) / ctas);
+  for (int q = (int)((int64_t)pieces * cta / ctas) + warp; q < q1; q += kDownWarps) {
+    const int i = q / (parts * nb), pb = q % (parts * nb), p = pb / nb, r = pb % nb * 32 + lane;
     float sum = 0.f;
     if (r < at.rank) {
+      const uint32_t from = base + 4u * (i * pitch + p * rp + r);
       float part[kAdapterCluster];
 #pragma unroll
-      for (int v = 0; v < kAdapterCluster; ++v) part[v] = adapter_load(from[v] + 4u * (i * wide + p * rp + r));
+      for (int v = 0; v < kAdapterCluster; ++v) part[v] = v < ctas ? adapter_load(adapter_remote(from, v)) : 0.f;
       sum = part[0];
 #pragma unroll
-      for (int v = 1; v < kAdapterCluster; ++v) sum += part[v];
+      for (int v = 1; v < kAdapterCluster; ++v) {
+        if (v < ctas) sum += part[v];
+      }
       sum *= factor;
     }
     __nv_bfloat16 o[SPLIT];
@@ -286,109 +310,218 @@ __global__ void __launch_bounds__(THREADS, CTAS) __cluster_dims__(kAdapterCluste
   adapter_cluster_sync();      // nobody leaves while another CTA reads its sums
 }
 
-// RB > 0: b's numbers of RB blocks of 32 of the rank stay in registers for all the tile's tokens; 0: they are read again for every 16 tokens.
-template <typename TY, int SPLIT, int RB>
-__global__ void __launch_bounds__(kAdapterThreads, 2)
+// A warp takes `per_warp` units of 32 outputs of a tile of up to MT * 16 tokens. y and b come by cp.async into a queue of kUpDepth units in shared memory;
+// a lane reads back just what it asked for itself, so the queue needs no barrier: it only holds more loads on their way than registers would. h stays
+// in registers where it fits. RB: blocks
+// of 32 of the rank whose b passes through the queue; 0: b is read where it is used (ranks above 64).
+constexpr int kUpThreads = 128, kUpWarps = kUpThreads / 32, kUpDepth = 3;
+template <typename TY, int MT, int RB>
+struct UpCfg {
+  static constexpr int kVecs = sizeof(TY) / 2;                     // 16-byte pieces of eight outputs
+  static constexpr int kY = 2 * MT * kVecs, kPieces = kY + 4 * RB; // of a lane and unit
+  static constexpr int kSmem = kUpWarps * kUpDepth * kPieces * 512;
+};
+__device__ __forceinline__ void adapter_queue16(uint32_t smem, const void* gmem, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0) : "memory");   // zeros where there is nothing
+}
+__device__ __forceinline__ uint4 adapter_shared16(uint32_t smem) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem) : "memory");
+  return v;
+}
+template <typename TY, int SPLIT, int MT, int RB>
+__global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : (RB == 2 ? 2 : 3))
     adapters_up_kernel(TY* y, int64_t ldy, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ b, const int32_t* __restrict__ ranks,
-                       const int32_t* __restrict__ rows, const int32_t* __restrict__ tiles, int tokens, int listed, int slots, int tile_rows,
-                       const AdapterParts parts, int chunks, int R) {
+                       const int32_t* __restrict__ rows, const int32_t* __restrict__ tiles, int tokens, int listed, int slots, const AdapterParts parts,
+                       int per_warp, int chunks, int R) {
+  using Cfg = UpCfg<TY, MT, RB>;
+  constexpr int kVecs = Cfg::kVecs;
+  extern __shared__ __align__(16) unsigned char queue[];
   pdl_launch_dependents();
-  const AdapterTile at = adapter_tile(tiles, blockIdx.x / chunks, ranks, tile_rows, listed, slots, R);
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const uint4 zero = make_uint4(0, 0, 0, 0);
-  // this warp's 32 outputs: units of 32 of each part, one part after the other
-  int p = 0, begin = 0, unit = blockIdx.x % chunks * (kAdapterThreads / 32) + (threadIdx.x >> 5);
-  while (p < parts.n) {
-    const int here = (parts.end[p] - begin + 31) / 32;
-    if (unit < here) break;
-    unit -= here;
+  const AdapterTile at = adapter_tile(tiles, blockIdx.x / chunks, ranks, MT * 16, listed, slots, R);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  // the part that this CTA's units of 32 outputs belong to, and this warp's
+  int p = 0, begin = 0, chunk = blockIdx.x % chunks, units = 0;
+  while (true) {
+    units = (parts.end[p] - begin + 31) / 32;
+    const int here = (units + per_warp * kUpWarps - 1) / (per_warp * kUpWarps);
+    if (chunk < here || p == parts.n - 1) break;
+    chunk -= here;
     begin = parts.end[p++];
   }
-  if (at.rank == 0 || p == parts.n) {
+  const int first = (chunk * kUpWarps + warp) * per_warp, mine = at.rank == 0 ? 0 : min(per_warp, units - first), end = parts.end[p];
+  if (mine <= 0) {
     pdl_wait();
     return;
   }
-  const int n0 = begin + unit * 32, end = parts.end[p], n = n0 + 8 * c, r32 = (R + 31) & ~31, line = parts.n * r32;   // n: this lane's eight outputs
+  const int r32 = (R + 31) & ~31, line = parts.n * r32, last = at.first + at.rows;
+  const uint32_t lane_queue = (uint32_t)__cvta_generic_to_shared(queue) + (uint32_t)(warp * kUpDepth * Cfg::kPieces * 512 + lane * 16);
+  int n0 = begin + first * 32;                              // the next unit to be multiplied; this lane's eight outputs begin 8 c further on
+  int ask_b_n = n0, ask_y_n = n0, ask_b_at = 0, ask_y_at = 0, at_slot = 0;   // the next to be asked for, and their places in the queue
+  const int col_of = (g >> 1) * 8 + (g & 1);                // + 2 t: the row of b for the t-th instruction
   b += (int64_t)at.slot * parts.end[parts.n - 1] * R + 8 * c;
-  auto load_b = [&](int r0, uint4 (&bv)[4]) {
+  auto next = [&](int& slot) { slot = slot == kUpDepth - 1 ? 0 : slot + 1; };
+  auto ask_b = [&]() {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int col = n0 + (g >> 1) * 8 + 2 * t + (g & 1), left = at.rank - (r0 + 8 * c);
-      bv[t] = col < end && left > 0 ? adapter_first(adapter_load16(b + (int64_t)col * R + r0), left) : zero;
+    for (int v = 0; v < RB; ++v) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int col = ask_b_n + col_of + 2 * t;
+        const bool in = col < end && 32 * v + 8 * c < at.rank;
+        adapter_queue16(lane_queue + (uint32_t)((ask_b_at * Cfg::kPieces + Cfg::kY + 4 * v + t) * 512), in ? b + (int64_t)col * R + 32 * v : b, in);
+      }
+    }
+    ask_b_n += 32;
+    next(ask_b_at);
+  };
+  TY* yr[2 * MT];
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) {
+    const int r = g + 8 * i < at.rows ? adapter_row(rows, at.first + g + 8 * i, tokens) : -1;
+    yr[i] = r >= 0 ? y + (int64_t)r * ldy + 8 * c : nullptr;
+  }
+  auto ask_y = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const bool in = yr[i] && ask_y_n + 8 * c < end;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v)
+        adapter_queue16(lane_queue + (uint32_t)((ask_y_at * Cfg::kPieces + i * kVecs + v) * 512), in ? yr[i] + ask_y_n + v * (8 / kVecs) : y, in);
+    }
+    ask_y_n += 32;
+    next(ask_y_at);
+    copy_commit();
+  };
+  // b is not written by any kernel: the first units' is on its way before the wait for h
+#pragma unroll
+  for (int i = 0; i < kUpDepth - 1; ++i) {
+    if (i < mine) ask_b();
+  }
+  pdl_wait();
+#pragma unroll
+  for (int i = 0; i < kUpDepth - 1; ++i) {
+    if (i < mine) {
+      ask_y();
+    } else {
+      copy_commit();
+    }
+  }
+  // h as the first operand of all the warp's units; tokens behind the tile's: any, they are not stored
+  constexpr bool kHeld = RB > 0 && MT * RB * SPLIT <= 16;
+  uint4 hv[kHeld ? MT : 1][kHeld ? RB : 1][SPLIT][2];
+  auto load_h = [&](uint4 (&o)[SPLIT][2], int m, int r0) {
+#pragma unroll
+    for (int v = 0; v < SPLIT; ++v) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = min(at.first + m * 16 + g + 8 * e, last - 1);
+        o[v][e] = adapter_load16_new(h + ((int64_t)v * listed + i) * line + p * r32 + r0 + 8 * c);
+      }
     }
   };
-  constexpr int kVecs = sizeof(TY) / 2, kAhead = 4;       // 16-byte pieces of eight outputs; tiles of 16 tokens whose y is on its way
-  uint4 bv[RB > 0 ? RB : 1][4];
+  if constexpr (kHeld) {
 #pragma unroll
-  for (int i = 0; i < RB; ++i) load_b(32 * i, bv[i]);
-  const int last = at.first + at.rows;
-  int row[2 * kAhead];
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-  for (int i = 0; i < 2 * kAhead; ++i) row[i] = g + 8 * i < at.rows && n < end ? adapter_row(rows, at.first + g + 8 * i, tokens) : -1;
-  pdl_wait();
-  uint4 yv[2 * kAhead][kVecs];
-#pragma unroll
-  for (int i = 0; i < 2 * kAhead; ++i) {
-#pragma unroll
-    for (int v = 0; v < kVecs; ++v) yv[i][v] = row[i] >= 0 ? adapter_load16(y + (int64_t)row[i] * ldy + n + v * (8 / kVecs)) : zero;
-  }
-#pragma unroll
-  for (int m = 0; m < kAhead; ++m) {
-    if (m * 16 >= at.rows) break;
-    float acc[4][4] = {};
-    const int h0 = min(at.first + m * 16 + g, last - 1), h1 = min(at.first + m * 16 + g + 8, last - 1);   // rows behind the tile's: any, they are not stored
-    auto multiply = [&](int r0, const uint4 (&bb)[4]) {
-#pragma unroll
-      for (int v = 0; v < SPLIT; ++v) {
-        const __nv_bfloat16* hv = h + (int64_t)v * listed * line + p * r32 + r0 + 8 * c;
-        const uint4 u0 = adapter_load16(hv + (int64_t)h0 * line), u1 = adapter_load16(hv + (int64_t)h1 * line);
-        const uint32_t lo[4] = {u0.x, u1.x, u0.y, u1.y}, hi[4] = {u0.z, u1.z, u0.w, u1.w};
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          mma_bf16(acc[t], lo, bb[t].x, bb[t].y);
-          mma_bf16(acc[t], hi, bb[t].z, bb[t].w);
-        }
-      }
-    };
-    if (RB > 0) {
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        if (32 * i < at.rank) multiply(32 * i, bv[i]);
-      }
-    } else {
-#pragma unroll 1
-      for (int r0 = 0; r0 < at.rank; r0 += 32) {
-        load_b(r0, bv[0]);
-        multiply(r0, bv[0]);
+      for (int v = 0; v < RB; ++v) {
+        if (32 * v < at.rank) load_h(hv[m][v], m, 32 * v);
       }
     }
+  }
+#pragma unroll 1
+  for (int u = 0; u < mine; ++u, n0 += 32) {
+    if (u + kUpDepth - 1 < mine) {
+      ask_b();
+      ask_y();
+    } else {
+      copy_commit();
+    }
+    copy_wait<kUpDepth - 1>();
+    const uint32_t from = lane_queue + (uint32_t)(at_slot * Cfg::kPieces * 512);
+    next(at_slot);
+    uint4 bv[RB > 0 ? RB : 1][4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = 2 * m + e;
-      if (row[i] < 0) continue;
-      TY* to = y + (int64_t)row[i] * ldy + n;
+    for (int v = 0; v < RB; ++v) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) bv[v][t] = adapter_shared16(from + (Cfg::kY + 4 * v + t) * 512);
+      if (at.rank < 32 * (v + 1)) {     // the slot's rank ends in this block
+#pragma unroll
+        for (int t = 0; t < 4; ++t) bv[v][t] = adapter_first(bv[v][t], at.rank - (32 * v + 8 * c));
+      }
+    }
+    const bool stored = n0 + 8 * c < end;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if (m * 16 >= at.rows) break;
+      // the sums begin at y where that is bfloat16 (a unit in their 24th bit is far below its rounding), else at zero
+      float acc[4][4];
       if constexpr (sizeof(TY) == 2) {
-        const uint32_t w[4] = {yv[i][0].x, yv[i][0].y, yv[i][0].z, yv[i][0].w};
-        float o[8];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) o[2 * t] = acc[t][2 * e] + __uint_as_float(w[t] << 16), o[2 * t + 1] = acc[t][2 * e + 1] + __uint_as_float(w[t] & 0xffff0000u);
-        Vec<TY>::store(to, o);
+        for (int e = 0; e < 2; ++e) {
+          const uint4 yv = adapter_shared16(from + (2 * m + e) * 512);
+          const uint32_t w[4] = {yv.x, yv.y, yv.z, yv.w};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc[t][2 * e] = __uint_as_float(w[t] << 16), acc[t][2 * e + 1] = __uint_as_float(w[t] & 0xffff0000u);
+        }
       } else {
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          const float o[4] = {acc[2 * v][2 * e] + __uint_as_float(yv[i][v].x), acc[2 * v][2 * e + 1] + __uint_as_float(yv[i][v].y),
-                              acc[2 * v + 1][2 * e] + __uint_as_float(yv[i][v].z), acc[2 * v + 1][2 * e + 1] + __uint_as_float(yv[i][v].w)};
-          Vec<TY>::store(to + 4 * v, o);
+        for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      }
+      auto multiply = [&](const uint4 (&hh)[SPLIT][2], const uint4 (&bb)[4]) {
+#pragma unroll
+        for (int v = 0; v < SPLIT; ++v) {
+          const uint32_t lo[4] = {hh[v][0].x, hh[v][1].x, hh[v][0].y, hh[v][1].y}, hi[4] = {hh[v][0].z, hh[v][1].z, hh[v][0].w, hh[v][1].w};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            mma_bf16(acc[t], lo, bb[t].x, bb[t].y);
+            mma_bf16(acc[t], hi, bb[t].z, bb[t].w);
+          }
+        }
+      };
+      if constexpr (kHeld) {
+#pragma unroll
+        for (int v = 0; v < RB; ++v) {
+          if (32 * v < at.rank) multiply(hv[m][v], bv[v]);
+        }
+      } else if constexpr (RB > 0) {
+#pragma unroll
+        for (int v = 0; v < RB; ++v) {
+          if (32 * v < at.rank) {
+            load_h(hv[0][0], m, 32 * v);
+            multiply(hv[0][0], bv[v]);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int r0 = 0; r0 < at.rank; r0 += 32) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int col = n0 + col_of + 2 * t, left = at.rank - (r0 + 8 * c);
+            bv[0][t] = col < end && left > 0 ? adapter_first(adapter_load16(b + (int64_t)col * R + r0), left) : make_uint4(0, 0, 0, 0);
+          }
+          load_h(hv[0][0], m, r0);
+          multiply(hv[0][0], bv[0]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        TY* to = yr[2 * m + e];
+        if (!to || !stored) continue;
+        if constexpr (sizeof(TY) == 2) {
+          const float o[8] = {acc[0][2 * e], acc[0][2 * e + 1], acc[1][2 * e], acc[1][2 * e + 1], acc[2][2 * e], acc[2][2 * e + 1], acc[3][2 * e], acc[3][2 * e + 1]};
+          Vec<TY>::store(to + n0, o);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            const uint4 yv = adapter_shared16(from + (2 * (2 * m + e) + v) * 512);
+            const float o[4] = {acc[2 * v][2 * e] + __uint_as_float(yv.x), acc[2 * v][2 * e + 1] + __uint_as_float(yv.y),
+                                acc[2 * v + 1][2 * e] + __uint_as_float(yv.z), acc[2 * v + 1][2 * e + 1] + __uint_as_float(yv.w)};
+            Vec<TY>::store(to + n0 + 4 * v, o);
+          }
         }
       }
     }
   }
-}
-
-// Shared memory of adapters_down_kernel: eight (or sixteen) warps along k while G tiles cover a's rows; then wn of them side by side, wn * G < 2 * tiles.
-static size_t adapter_down_smem(int tiles, int mt, int g, int warps) {
-  const int wide = 8 * (tiles <= g ? warps * tiles : (tiles > warps * g ? tiles : warps * g));
-  return (size_t)wide * mt * 16 * 4;
 }
 
 struct AdapterCall {
@@ -405,29 +538,54 @@ struct AdapterCall {
   cudaStream_t stream;
 };
 
-template <int SPLIT, int MT, int G, int THREADS, int CTAS>
+template <int SPLIT, int MT, int G>
 static void launch_adapters_down(const AdapterCall& q) {
-  const size_t smem = adapter_down_smem(q.parts.n * ((q.rank + 7) / 8), MT, G, THREADS / 32);
-  auto kernel = adapters_down_kernel<SPLIT, MT, G, THREADS, CTAS>;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  launch_kernel(kernel, dim3(q.n_tiles * kAdapterCluster), dim3(THREADS), smem, q.stream, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tokens, q.listed,
-                q.slots, q.parts.n, q.rank, q.inputs);
+  // sums of h: sixteen warps' while G tiles cover a's rows, else those of the warps that share a group (at most 16 groups of G)
+  const int tiles = q.parts.n * ((q.rank + 7) / 8);
+  // (a slot of a smaller rank has more warps along k), each row up to 24 floats longer than its numbers
+  const size_t smem = (size_t)kDownWarps * ((tiles <= G ? tiles : G) * 8 + 24) * MT * 16 * sizeof(float);
+  static_assert(kDownWarps * G * 8 >= kAdapterMaxWidth, "one round of groups covers h");
+  auto kernel = adapters_down_kernel<SPLIT, MT, G>;
+  if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // as many CTAs a tile as still run all at once, one a processor
+  int ctas = kAdapterCluster;
+  while (ctas > 1 && (int64_t)q.n_tiles * ctas > processors()) ctas /= 2;
+  launch_kernel_cluster(kernel, dim3(q.n_tiles * ctas), dim3(kDownThreads), smem, q.stream, ctas, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tokens,
+                        q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas);
+}
+template <typename TY, int SPLIT, int MT, int RB>
+static void launch_adapters_up(const AdapterCall& q, int units) {
+  constexpr int kSmem = UpCfg<TY, MT, RB>::kSmem;
+  auto kernel = adapters_up_kernel<TY, SPLIT, MT, RB>;
+  if (kSmem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  // units of a warp: up to 8, as few as leave every processor about twelve warps
+  int64_t per_warp = (int64_t)units * q.n_tiles / (12 * (int64_t)processors());
+  per_warp = per_warp < 1 ? 1 : (per_warp > 8 ? 8 : per_warp);
+  int chunks = 0;
+  for (int p = 0; p < q.parts.n; ++p) {
+    const int here = (q.parts.end[p] - (p ? q.parts.end[p - 1] : 0) + 31) / 32;
+    chunks += (here + (int)per_warp * kUpWarps - 1) / ((int)per_warp * kUpWarps);
+  }
+  launch_kernel(kernel, dim3(q.n_tiles * chunks), dim3(kUpThreads), kSmem, q.stream, (TY*)q.y, q.ldy, q.h, q.b, q.ranks, q.rows, q.tiles, q.tokens, q.listed, q.slots,
+                q.parts, (int)per_warp, chunks, q.rank);
 }
 template <typename TY, int SPLIT>
-static int launch_adapters(const AdapterCall& q) {
-  if (q.tile_rows <= 16) {
-    launch_adapters_down<SPLIT, 1, 4, 512, 2>(q);
+static int launch_adapters(const AdapterCall& q, int units) {
+  const bool few = q.tile_rows <= 16;
+  if (few) {
+    launch_adapters_down<SPLIT, 1, 8>(q);
   } else {
-    launch_adapters_down<SPLIT, 4, 4, 256, 2>(q);
+    launch_adapters_down<SPLIT, 4, 4>(q);
   }
   int rc = check_launch("adapters_add");
   if (rc != ROOST_OK) return rc;
-  int units = 0;
-  for (int p = 0; p < q.parts.n; ++p) units += (q.parts.end[p] - (p ? q.parts.end[p - 1] : 0) + 31) / 32;
-  const int chunks = (units + kAdapterThreads / 32 - 1) / (kAdapterThreads / 32);
-  auto kernel = q.rank <= 32 ? adapters_up_kernel<TY, SPLIT, 1> : (q.rank <= 64 ? adapters_up_kernel<TY, SPLIT, 2> : adapters_up_kernel<TY, SPLIT, 0>);
-  launch_kernel(kernel, dim3(q.n_tiles * chunks), dim3(kAdapterThreads), 0, q.stream, (TY*)q.y, q.ldy, q.h, q.b, q.ranks, q.rows, q.tiles, q.tokens, q.listed, q.slots,
-                q.tile_rows, q.parts, chunks, q.rank);
+  if (q.rank <= 32) {
+    few ? launch_adapters_up<TY, SPLIT, 1, 1>(q, units) : launch_adapters_up<TY, SPLIT, 4, 1>(q, units);
+  } else if (q.rank <= 64) {
+    few ? launch_adapters_up<TY, SPLIT, 1, 2>(q, units) : launch_adapters_up<TY, SPLIT, 4, 2>(q, units);
+  } else {
+    few ? launch_adapters_up<TY, SPLIT, 1, 0>(q, units) : launch_adapters_up<TY, SPLIT, 4, 0>(q, units);
+  }
   return check_launch("adapters_add");
 }
 
@@ -475,11 +633,11 @@ extern "C" int roost_adapters_add(void* y, int64_t ldy, const void* x, int64_t l
     ROOST_REQUIRE(h, "adapters_add: the workspace is missing");
     int64_t units = 0;
     for (int p = 0; p < n_parts; ++p) units += (widths[p] + 31) / 32;
-    if ((units + 7) / 8 * n_tiles > 2147483647LL) return fail(ROOST_ERR_UNSUPPORTED, "adapters_add: too many tiles");
+    if (units * n_tiles > 2147483647LL) return fail(ROOST_ERR_UNSUPPORTED, "adapters_add: too many tiles");
     const AdapterCall q{y,    ldy,     (const __nv_bfloat16*)x, ldx,       (const __nv_bfloat16*)a, (const __nv_bfloat16*)b, (__nv_bfloat16*)h, scales, ranks,
                         rows, tiles, n_tiles,                 tile_rows, listed,                  tokens,                  slots,             rank,   inputs,
                         parts, (cudaStream_t)stream};
-    return y_dtype == ROOST_BF16 ? launch_adapters<__nv_bfloat16, 2>(q) : launch_adapters<float, 3>(q);
+    return y_dtype == ROOST_BF16 ? launch_adapters<__nv_bfloat16, 2>(q, (int)units) : launch_adapters<float, 3>(q, (int)units);
   }
   const size_t smem = (size_t)tile_rows * n_parts * rank * sizeof(float);
   ROOST_DISPATCH_DTYPE(dtype, T, ROOST_DISPATCH_DTYPE(y_dtype, TY, {
