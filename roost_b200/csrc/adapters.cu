@@ -162,6 +162,10 @@ __device__ __forceinline__ uint4 adapter_first(uint4 v, int n) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+__device__ __forceinline__ void adapter_queue16(uint32_t smem, const void* gmem, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0) : "memory");   // zeros where there is nothing
+}
+
 struct AdapterTile {
   int slot, first, rows, rank;   // rank 0: nothing to do
 };
@@ -179,19 +183,43 @@ __device__ __forceinline__ int adapter_row(const int32_t* rows, int at, int toke
   return r >= 0 && r < tokens ? r : -1;
 }
 
-// A cluster of `ctas` takes a tile of up to MT * 16 tokens, CTA v the v-th part of k. Sixteen warps, one CTA a processor: warps side by side on groups of G
-// tiles of 8 rows of a, and on k with what is left of them; a warp's loads of a block of 32 of k (2 MT of x, G of a) are on their way together, a's for
-// the next block as soon as the products have read this one's. h [SPLIT][listed][parts * r32], r32 = R rounded up to 32.
-constexpr int kDownThreads = 512, kDownWarps = kDownThreads / 32;
-template <int SPLIT, int MT, int G>
-__global__ void __launch_bounds__(kDownThreads, 1)
+// A cluster of `ctas` takes a tile of up to MT * 16 tokens, CTA v the v-th part of k, SK of k a stage: x's and a's rows by cp.async, whole lines of memory,
+// into swizzled rows of shared memory, as many stages as fit on their way, a's first ones ahead of the wait for x. Where all of a CTA's blocks fit
+// there is one wait for all of them. A thread copies the same pieces of the same rows in every stage, so that its addresses stay in registers. Warps: KG
+// along the steps of 16 of k, whose sums are added up afterwards, NS side by side on a's rows, NP pairs of tiles of 8 each, and two on the tokens of
+// MT 4. What a stage costs is instructions, not bytes: with a warp 16 x 16 of the products, 64 of k a stage and addresses formed for each it took
+// 0.55 us for 10 and for 16 KB alike.
+// h [SPLIT][listed][parts * r32], r32 = R rounded up to 32.
+template <int MT, int KG, int NS, int NP, int SK>
+struct DownCfg {
+  static constexpr int kRowsX = MT * 16, kMw = MT == 4 ? 2 : 1;          // tokens of a tile; tiles of 16 of them a warp
+  static constexpr int kWarps = KG * NS * (MT / kMw), kThreads = kWarps * 32;
+  static constexpr int kWide = NS * NP * 16;                             // rows of a at most
+  static constexpr int kRowBytes = SK * 2, kPieces = SK / 8, kPass = kThreads / kPieces, kPasses = (kRowsX + kWide + kPass - 1) / kPass;
+  static constexpr int kCtas = kThreads == 256 && kWide <= 192 ? 2 : 1;   // a processor
+};
+__device__ __forceinline__ void adapter_wait_stages(int in_flight) {
+  switch (in_flight) {
+    case 0: copy_wait<0>(); break;
+    case 1: copy_wait<1>(); break;
+    case 2: copy_wait<2>(); break;
+    case 3: copy_wait<3>(); break;
+    case 4: copy_wait<4>(); break;
+    case 5: copy_wait<5>(); break;
+    default: copy_wait<6>(); break;
+  }
+}
+template <int SPLIT, int MT, int KG, int NS, int NP, int SK>
+__global__ void __launch_bounds__(DownCfg<MT, KG, NS, NP, SK>::kThreads, DownCfg<MT, KG, NS, NP, SK>::kCtas)
     adapters_down_kernel(__nv_bfloat16* __restrict__ h_out, const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ a,
                          const float* __restrict__ scales, const int32_t* __restrict__ ranks, const int32_t* __restrict__ rows, const int32_t* __restrict__ tiles,
-                         int tokens, int listed, int slots, int parts, int R, int K, int ctas) {
-  extern __shared__ __align__(16) float h[];     // [warps along k][tokens of the tile][parts * rank, in whole tiles of 8, and what fills the pitch]
+                         int tokens, int listed, int slots, int parts, int R, int K, int ctas, int stages, int stage_bytes) {
+  using Cfg = DownCfg<MT, KG, NS, NP, SK>;
+  constexpr int kRowsX = Cfg::kRowsX, kThreads = Cfg::kThreads, kWarps = Cfg::kWarps, kMw = Cfg::kMw, kPasses = Cfg::kPasses;
+  extern __shared__ __align__(1024) unsigned char smem[];
   pdl_launch_dependents();
   const int cta = (int)adapter_cluster_rank();
-  const AdapterTile at = adapter_tile(tiles, blockIdx.x / ctas, ranks, MT * 16, listed, slots, R);
+  const AdapterTile at = adapter_tile(tiles, blockIdx.x / ctas, ranks, kRowsX, listed, slots, R);
   if (at.rank == 0) {    // the whole cluster
     pdl_wait();
     return;
@@ -200,94 +228,109 @@ __global__ void __launch_bounds__(kDownThreads, 1)
   const int nt = (at.rank + 7) / 8, rp = 8 * nt, wide = parts * rp, n_tiles = parts * nt;
   const int pitch = wide + ((40 - wide % 32) & 31);     // floats of a token's sums: 8 beyond a multiple of 32, so that a warp's stores meet all banks
   const float factor = scales[at.slot];
-  // Rows that do not exist (tokens behind the tile's, ranks behind the slot's) are read from ones that do: each makes numbers of its own row of h only,
-  // and those are not used.
-  const __nv_bfloat16* xr[2 * MT];
+  // Where this thread's rows of a stage come from, x's and behind them a's. Rows that do not exist (tokens behind the tile's, ranks behind the slot's) are
+  // read from ones that do: each makes numbers of its own row or column of h only, and those are not used.
+  const int piece = threadIdx.x % Cfg::kPieces, row0 = threadIdx.x / Cfg::kPieces;
+  const __nv_bfloat16* source[kPasses];
 #pragma unroll
-  for (int i = 0; i < 2 * MT; ++i) xr[i] = x + (int64_t)max(adapter_row(rows, at.first + min(g + 8 * i, at.rows - 1), tokens), 0) * ldx + 8 * c;
-  const int groups = min((n_tiles + G - 1) / G, kDownWarps), wk = kDownWarps / groups, my_k = warp / groups;
-  const int blocks = (K + 31) / 32, whole = K / 32;
-  const int kb0 = (int)((int64_t)blocks * cta / ctas) + my_k, kb1 = my_k < wk ? (int)((int64_t)blocks * (cta + 1) / ctas) : 0;
-  a += (int64_t)at.slot * parts * R * K;
-  bool waited = false;
-  for (int t0 = warp % groups * G; t0 < n_tiles; t0 += groups * G) {
-    float acc[MT][G][4] = {};
-    const __nv_bfloat16* ar[G];
+  for (int i = 0; i < kPasses; ++i) {
+    const int row = row0 + i * Cfg::kPass, j = max(row - kRowsX, 0);
+    source[i] = row < kRowsX ? x + (int64_t)max(adapter_row(rows, at.first + min(row, at.rows - 1), tokens), 0) * ldx
+                             : a + (((int64_t)at.slot * parts + min(j / rp, parts - 1)) * R + min(j % rp, at.rank - 1)) * K;
+  }
+  const int blocks = (K + SK - 1) / SK, kb0 = (int)((int64_t)blocks * cta / ctas), count = (int)((int64_t)blocks * (cta + 1) / ctas) - kb0;   // of this CTA
+  const uint32_t base = (uint32_t)__cvta_generic_to_shared(smem), mine = base + swizzled<Cfg::kRowBytes>(row0, piece);
+  static_assert(Cfg::kPass % 8 == 0, "a thread's rows have one swizzle");
+  auto ask = [&](int block, int stage, int from, int to) {     // rows [from, to) of one of this CTA's blocks
+    const int k = (kb0 + block) * SK + piece * 8;
+    const bool in = k < K;
 #pragma unroll
-    for (int t = 0; t < G; ++t) {
-      const int tt = min(t0 + t, n_tiles - 1), r = min(tt % nt * 8 + g, at.rank - 1);
-      ar[t] = a + ((int64_t)(tt / nt) * R + r) * K + 8 * c;
+    for (int i = 0; i < kPasses; ++i) {
+      const int row = row0 + i * Cfg::kPass;
+      if (row >= from && row < to) adapter_queue16(mine + stage * stage_bytes + i * Cfg::kPass * Cfg::kRowBytes, source[i] + (in ? k : 0), in);
     }
-    uint4 xv[2 * MT], av[G];
-    auto multiply = [&]() {
+  };
+  const bool resident = count <= stages;
+  const int first = resident ? count : stages - 1;               // blocks asked for ahead of the loop
+  for (int i = 0; i < first; ++i) ask(i, i, kRowsX, kRowsX + wide);
+  pdl_wait();
+  for (int i = 0; i < first; ++i) {
+    ask(i, i, 0, kRowsX);
+    copy_commit();
+  }
+  if (resident) {
+    copy_wait<0>();
+    __syncthreads();
+  }
+  const int kg = warp % KG, wn = warp / KG % NS, m0 = warp / (KG * NS) * kMw * 16;
+  float acc[kMw][NP][2][4] = {};
+  int stage = 0, ahead = stages - 1;
+  for (int block = 0; block < count; ++block) {
+    if (!resident) {
+      adapter_wait_stages(stages - 2);
+      __syncthreads();      // every thread's copies of this stage have come, and the one asked for next has been read by all
+      if (block + stages - 1 < count) ask(block + stages - 1, ahead, 0, kRowsX + wide);
+      copy_commit();
+      ahead = ahead == stages - 1 ? 0 : ahead + 1;
+    }
+    const uint32_t sx = base + stage * stage_bytes;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint32_t lo[4] = {xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y}, hi[4] = {xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w};
+    for (int step = 0; step < SK / 16; step += KG) {
+      uint32_t av[kMw][4];
 #pragma unroll
-        for (int t = 0; t < G; ++t) {
-          mma_bf16(acc[m][t], lo, av[t].x, av[t].y);
-          mma_bf16(acc[m][t], hi, av[t].z, av[t].w);
+      for (int m = 0; m < kMw; ++m) ldsm_x4(av[m], sx + swizzled<Cfg::kRowBytes>(m0 + m * 16 + (lane & 15), (step + kg) * 2 + (lane >> 4)));
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int q = wn + NS * i;     // this pair of tiles of 8
+        if (2 * q >= n_tiles) break;
+        uint32_t bv[4];
+        ldsm_x4(bv, sx + swizzled<Cfg::kRowBytes>(kRowsX + q * 16 + ((lane >> 4) << 3) + (lane & 7), (step + kg) * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int m = 0; m < kMw; ++m) {
+          mma_bf16(acc[m][i][0], av[m], bv[0], bv[1]);
+          mma_bf16(acc[m][i][1], av[m], bv[2], bv[3]);
         }
       }
-    };
-    auto fetch_a = [&](int kb) {
-      if (kb < min(kb1, whole)) {
-#pragma unroll
-        for (int t = 0; t < G; ++t) av[t] = adapter_load16(ar[t] + kb * 32);
-      }
-    };
-    fetch_a(kb0);
-    if (!waited) pdl_wait();
-    waited = true;
-    int kb = kb0;
-#pragma unroll 1
-    for (; kb < min(kb1, whole); kb += wk) {
-#pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) xv[i] = adapter_load16(xr[i] + kb * 32);
-      multiply();
-      fetch_a(kb + wk);
     }
-    if (kb < kb1) {      // the last block where K is no multiple of 32: zeros behind its end in both
-      const bool in = kb * 32 + 8 * c < K;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
+    stage = stage == stages - 1 ? 0 : stage + 1;
+  }
+  copy_wait<0>();
+  __syncthreads();
+  // the sums over the stages: [KG][tokens of the tile][pitch]
+  float* h = reinterpret_cast<float*>(smem);
 #pragma unroll
-      for (int t = 0; t < G; ++t) av[t] = in ? adapter_load16(ar[t] + kb * 32) : zero;
+  for (int i = 0; i < NP; ++i) {
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) xv[i] = in ? adapter_load16(xr[i] + kb * 32) : zero;
-      multiply();
-    }
-    if (my_k < wk) {
+    for (int t = 0; t < 2; ++t) {
+      const int tile = 2 * (wn + NS * i) + t;
+      if (tile >= n_tiles) continue;
 #pragma unroll
-      for (int t = 0; t < G; ++t) {
-        if (t0 + t >= n_tiles) continue;
+      for (int m = 0; m < kMw; ++m) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = m * 16 + g + 8 * e;
-            if (i < at.rows) *reinterpret_cast<float2*>(h + (my_k * at.rows + i) * pitch + (t0 + t) * 8 + 2 * c) = make_float2(acc[m][t][2 * e], acc[m][t][2 * e + 1]);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int row = m0 + m * 16 + g + 8 * e;
+          if (row < at.rows) *reinterpret_cast<float2*>(h + (kg * at.rows + row) * pitch + tile * 8 + 2 * c) = make_float2(acc[m][i][t][2 * e], acc[m][i][t][2 * e + 1]);
         }
       }
     }
   }
-  if (!waited) pdl_wait();
-  const int count = at.rows * pitch;
-  if (wk > 1) {
+  if constexpr (KG > 1) {
     __syncthreads();
-    for (int e = threadIdx.x; e < count; e += kDownThreads) {
-      float sum = h[e];
-#pragma unroll 4
-      for (int v = 1; v < wk; ++v) sum += h[v * count + e];
-      h[e] = sum;
+    const int all = at.rows * pitch;
+    for (int e = threadIdx.x; e < all; e += kThreads) {
+      float part[KG];
+#pragma unroll
+      for (int v = 0; v < KG; ++v) part[v] = h[v * all + e];
+#pragma unroll
+      for (int v = 1; v < KG; ++v) part[0] += part[v];
+      h[e] = part[0];
     }
   }
   adapter_cluster_sync();
   // a warp 32 numbers of a token's part at a time, a CTA its share of them
   const int r32 = (R + 31) & ~31, nb = (at.rank + 31) / 32, pieces = at.rows * parts * nb;
-  const uint32_t base = (uint32_t)__cvta_generic_to_shared(h);
   const int q1 = (int)((int64_t)pieces * (cta + 1) / ctas);
-  for (int q = (int)((int64_t)pieces * cta / ctas) + warp; q < q1; q += kDownWarps) {
+  for (int q = (int)((int64_t)pieces * cta / ctas) + warp; q < q1; q += kWarps) {
     const int i = q / (parts * nb), pb = q % (parts * nb), p = pb / nb, r = pb % nb * 32 + lane;
     float sum = 0.f;
     if (r < at.rank) {
@@ -321,9 +364,6 @@ struct UpCfg {
   static constexpr int kY = 2 * MT * kVecs, kPieces = kY + 4 * RB; // of a lane and unit
   static constexpr int kSmem = kUpWarps * kUpDepth * kPieces * 512;
 };
-__device__ __forceinline__ void adapter_queue16(uint32_t smem, const void* gmem, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0) : "memory");   // zeros where there is nothing
-}
 __device__ __forceinline__ uint4 adapter_shared16(uint32_t smem) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem) : "memory");
@@ -538,20 +578,30 @@ struct AdapterCall {
   cudaStream_t stream;
 };
 
-template <int SPLIT, int MT, int G>
+template <int SPLIT, int MT, int KG, int NS, int NP, int SK>
 static void launch_adapters_down(const AdapterCall& q) {
-  // sums of h: sixteen warps' while G tiles cover a's rows, else those of the warps that share a group (at most 16 groups of G)
-  const int tiles = q.parts.n * ((q.rank + 7) / 8);
-  // (a slot of a smaller rank has more warps along k), each row up to 24 floats longer than its numbers
-  const size_t smem = (size_t)kDownWarps * ((tiles <= G ? tiles : G) * 8 + 24) * MT * 16 * sizeof(float);
-  static_assert(kDownWarps * G * 8 >= kAdapterMaxWidth, "one round of groups covers h");
-  auto kernel = adapters_down_kernel<SPLIT, MT, G>;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  // as many CTAs a tile as still run all at once, one a processor
-  int ctas = kAdapterCluster;
-  while (ctas > 1 && (int64_t)q.n_tiles * ctas > processors()) ctas /= 2;
-  launch_kernel_cluster(kernel, dim3(q.n_tiles * ctas), dim3(kDownThreads), smem, q.stream, ctas, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tokens,
-                        q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas);
+  using Cfg = DownCfg<MT, KG, NS, NP, SK>;
+  // As many CTAs a tile as run all at once. A cluster's CTAs lie in one group of processors, so clusters of eight and four leave some of every group
+  // alone: 15 of eight and 33 of four fit the 148 processors at a CTA each, 33 and 71 at two (sixteen of eight at one took two turns, 16 us for 7.6).
+  const int percent[4] = {100, 100, Cfg::kCtas == 1 ? 90 : 95, Cfg::kCtas == 1 ? 80 : 88};
+  int log_ctas = 3;
+  while (log_ctas > 0 && ((int64_t)q.n_tiles << log_ctas) * 100 > (int64_t)percent[log_ctas] * Cfg::kCtas * processors()) --log_ctas;
+  const int ctas = 1 << log_ctas;
+  const int wide = q.parts.n * ((q.rank + 7) & ~7), blocks = ((q.inputs + SK - 1) / SK + ctas - 1) / ctas;
+  const int stage = (Cfg::kRowsX + ((wide + 15) & ~15)) * Cfg::kRowBytes, room = (Cfg::kCtas == 2 ? 104 : 208) * 1024;
+  int stages = room / stage;
+  if (stages >= blocks) {
+    stages = blocks;
+  } else if (stages > 8) {
+    stages = 8;      // copies of seven stages are told apart
+  }
+  if (stages < 2) stages = 2;
+  const size_t sums = (size_t)KG * Cfg::kRowsX * (wide + 31) * sizeof(float), all = (size_t)stages * stage;
+  const size_t smem = sums > all ? sums : all;
+  auto kernel = adapters_down_kernel<SPLIT, MT, KG, NS, NP, SK>;
+  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  launch_kernel_cluster(kernel, dim3(q.n_tiles * ctas), dim3(Cfg::kThreads), smem, q.stream, ctas, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tokens,
+                        q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas, stages, stage);
 }
 template <typename TY, int SPLIT, int MT, int RB>
 static void launch_adapters_up(const AdapterCall& q, int units) {
@@ -572,10 +622,24 @@ static void launch_adapters_up(const AdapterCall& q, int units) {
 template <typename TY, int SPLIT>
 static int launch_adapters(const AdapterCall& q, int units) {
   const bool few = q.tile_rows <= 16;
+  const int wide = q.parts.n * ((q.rank + 7) & ~7);
+  static_assert(kAdapterMaxWidth == 512, "the last forms cover all of h");
   if (few) {
-    launch_adapters_down<SPLIT, 1, 8>(q);
+    if (wide <= 32) {
+      launch_adapters_down<SPLIT, 1, 8, 1, 2, 128>(q);
+    } else if (wide <= 192) {
+      launch_adapters_down<SPLIT, 1, 4, 2, 6, 64>(q);
+    } else {
+      launch_adapters_down<SPLIT, 1, 1, 8, 4, 64>(q);
+    }
   } else {
-    launch_adapters_down<SPLIT, 4, 4>(q);
+    if (wide <= 64) {
+      launch_adapters_down<SPLIT, 4, 4, 2, 2, 128>(q);
+    } else if (wide <= 192) {
+      launch_adapters_down<SPLIT, 4, 2, 4, 3, 128>(q);
+    } else {
+      launch_adapters_down<SPLIT, 4, 1, 8, 4, 64>(q);
+    }
   }
   int rc = check_launch("adapters_add");
   if (rc != ROOST_OK) return rc;

@@ -734,7 +734,8 @@ struct Operands {
 int split_of(int64_t tiles, int k) {
   const int kbs = (k + kBlockK - 1) / kBlockK;
   int split = 8;
-  while (split > 1 && (tiles * split > processors() || split > kbs / 2)) split /= 2;
+  // clusters of eight and four leave some processors of every group alone: 15 and 33 of them fit 148 at a CTA each
+  while (split > 1 && (tiles * split * 100 > processors() * (int64_t)(split == 8 ? 80 : (split == 4 ? 88 : 100)) || split > kbs / 2)) split /= 2;
   return split;
 }
 
