@@ -353,16 +353,19 @@ __global__ void __launch_bounds__(DownCfg<MT, KG, NS, NP, SK>::kThreads, DownCfg
   adapter_cluster_sync();      // nobody leaves while another CTA reads its sums
 }
 
-// A warp takes `per_warp` units of 32 outputs of a tile of up to MT * 16 tokens. y and b come by cp.async into a queue of kUpDepth units in shared memory;
+// A warp takes `per_warp` units of 32 outputs of a tile, or of MT * 16 tokens of it. y and b come by cp.async into a queue of a few units in shared memory;
 // a lane reads back just what it asked for itself, so the queue needs no barrier: it only holds more loads on their way than registers would. h stays
 // in registers where it fits. RB: blocks
-// of 32 of the rank whose b passes through the queue; 0: b is read where it is used (ranks above 64).
-constexpr int kUpThreads = 128, kUpWarps = kUpThreads / 32, kUpDepth = 3;
+// of 32 of the rank whose b passes through the queue; 0: b is read where it is used (ranks above 64), a block of the rank for all the tokens.
+// Three units deep where 64 bfloat16 rows are a unit, two elsewhere: with less shared memory more CTAs, the next kernel's among them, find room (64 requests
+// over 32 adapters 16.6 us, 18.8 three deep; 2,048 float32 rows of 4,096 37.8, 48.2; but 4,001 bfloat16 rows of 24,576 93.5 two deep, 91.7 three).
+constexpr int kUpThreads = 128, kUpWarps = kUpThreads / 32;
 template <typename TY, int MT, int RB>
 struct UpCfg {
+  static constexpr int kDepth = sizeof(TY) == 2 && MT == 4 ? 3 : 2;
   static constexpr int kVecs = sizeof(TY) / 2;                     // 16-byte pieces of eight outputs
   static constexpr int kY = 2 * MT * kVecs, kPieces = kY + 4 * RB; // of a lane and unit
-  static constexpr int kSmem = kUpWarps * kUpDepth * kPieces * 512;
+  static constexpr int kSmem = kUpWarps * kDepth * kPieces * 512;
 };
 __device__ __forceinline__ uint4 adapter_shared16(uint32_t smem) {
   uint4 v;
@@ -370,15 +373,19 @@ __device__ __forceinline__ uint4 adapter_shared16(uint32_t smem) {
   return v;
 }
 template <typename TY, int SPLIT, int MT, int RB>
-__global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : (RB == 2 ? 2 : 3))
+__global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : 3)
     adapters_up_kernel(TY* y, int64_t ldy, const __nv_bfloat16* __restrict__ h, const __nv_bfloat16* __restrict__ b, const int32_t* __restrict__ ranks,
                        const int32_t* __restrict__ rows, const int32_t* __restrict__ tiles, int tokens, int listed, int slots, const AdapterParts parts,
-                       int per_warp, int chunks, int R) {
+                       int tile_rows, int subs, int per_warp, int chunks, int R) {
   using Cfg = UpCfg<TY, MT, RB>;
-  constexpr int kVecs = Cfg::kVecs;
+  constexpr int kVecs = Cfg::kVecs, kUpDepth = Cfg::kDepth;
   extern __shared__ __align__(16) unsigned char queue[];
   pdl_launch_dependents();
-  const AdapterTile at = adapter_tile(tiles, blockIdx.x / chunks, ranks, MT * 16, listed, slots, R);
+  AdapterTile at = adapter_tile(tiles, blockIdx.x / (chunks * subs), ranks, tile_rows, listed, slots, R);
+  const int sub = blockIdx.x / chunks % subs * MT * 16;      // this CTA's tokens of the tile
+  at.first += sub;
+  at.rows = min(at.rows - sub, MT * 16);
+  if (at.rows <= 0) at.rank = 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   // the part that this CTA's units of 32 outputs belong to, and this warp's
   int p = 0, begin = 0, chunk = blockIdx.x % chunks, units = 0;
@@ -447,7 +454,7 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : (RB == 2 ? 2 : 3))
     }
   }
   // h as the first operand of all the warp's units; tokens behind the tile's: any, they are not stored
-  constexpr bool kHeld = RB > 0 && MT * RB * SPLIT <= 16;
+  constexpr bool kHeld = RB > 0;
   uint4 hv[kHeld ? MT : 1][kHeld ? RB : 1][SPLIT][2];
   auto load_h = [&](uint4 (&o)[SPLIT][2], int m, int r0) {
 #pragma unroll
@@ -490,11 +497,8 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : (RB == 2 ? 2 : 3))
       }
     }
     const bool stored = n0 + 8 * c < end;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      if (m * 16 >= at.rows) break;
-      // the sums begin at y where that is bfloat16 (a unit in their 24th bit is far below its rounding), else at zero
-      float acc[4][4];
+    // the sums begin at y where that is bfloat16 (a unit in their 24th bit is far below its rounding), else at zero
+    auto begin_sums = [&](int m, float (&acc)[4][4]) {
       if constexpr (sizeof(TY) == 2) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -507,42 +511,19 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : (RB == 2 ? 2 : 3))
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
       }
-      auto multiply = [&](const uint4 (&hh)[SPLIT][2], const uint4 (&bb)[4]) {
+    };
+    auto multiply = [&](float (&acc)[4][4], const uint4 (&hh)[SPLIT][2], const uint4 (&bb)[4]) {
 #pragma unroll
-        for (int v = 0; v < SPLIT; ++v) {
-          const uint32_t lo[4] = {hh[v][0].x, hh[v][1].x, hh[v][0].y, hh[v][1].y}, hi[4] = {hh[v][0].z, hh[v][1].z, hh[v][0].w, hh[v][1].w};
+      for (int v = 0; v < SPLIT; ++v) {
+        const uint32_t lo[4] = {hh[v][0].x, hh[v][1].x, hh[v][0].y, hh[v][1].y}, hi[4] = {hh[v][0].z, hh[v][1].z, hh[v][0].w, hh[v][1].w};
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            mma_bf16(acc[t], lo, bb[t].x, bb[t].y);
-            mma_bf16(acc[t], hi, bb[t].z, bb[t].w);
-          }
-        }
-      };
-      if constexpr (kHeld) {
-#pragma unroll
-        for (int v = 0; v < RB; ++v) {
-          if (32 * v < at.rank) multiply(hv[m][v], bv[v]);
-        }
-      } else if constexpr (RB > 0) {
-#pragma unroll
-        for (int v = 0; v < RB; ++v) {
-          if (32 * v < at.rank) {
-            load_h(hv[0][0], m, 32 * v);
-            multiply(hv[0][0], bv[v]);
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int r0 = 0; r0 < at.rank; r0 += 32) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int col = n0 + col_of + 2 * t, left = at.rank - (r0 + 8 * c);
-            bv[0][t] = col < end && left > 0 ? adapter_first(adapter_load16(b + (int64_t)col * R + r0), left) : make_uint4(0, 0, 0, 0);
-          }
-          load_h(hv[0][0], m, r0);
-          multiply(hv[0][0], bv[0]);
+        for (int t = 0; t < 4; ++t) {
+          mma_bf16(acc[t], lo, bb[t].x, bb[t].y);
+          mma_bf16(acc[t], hi, bb[t].z, bb[t].w);
         }
       }
+    };
+    auto store = [&](int m, const float (&acc)[4][4]) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         TY* to = yr[2 * m + e];
@@ -560,6 +541,42 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : (RB == 2 ? 2 : 3))
           }
         }
       }
+    };
+    if constexpr (RB > 0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m * 16 >= at.rows) break;
+        float acc[4][4];
+        begin_sums(m, acc);
+#pragma unroll
+        for (int v = 0; v < RB; ++v) {
+          if (32 * v < at.rank) multiply(acc, hv[m][v], bv[v]);
+        }
+        store(m, acc);
+      }
+    } else {
+      float acc[MT][4][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) begin_sums(m, acc[m]);
+#pragma unroll 1
+      for (int r0 = 0; r0 < at.rank; r0 += 32) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int col = n0 + col_of + 2 * t, left = at.rank - (r0 + 8 * c);
+          bv[0][t] = col < end && left > 0 ? adapter_first(adapter_load16(b + (int64_t)col * R + r0), left) : make_uint4(0, 0, 0, 0);
+        }
+        load_h(hv[0][0], 0, r0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          uint4 now[SPLIT][2];
+#pragma unroll
+          for (int v = 0; v < SPLIT; ++v) now[v][0] = hv[0][0][v][0], now[v][1] = hv[0][0][v][1];
+          if (m + 1 < MT) load_h(hv[0][0], m + 1, r0);
+          multiply(acc[m], now, bv[0]);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) store(m, acc[m]);
     }
   }
 }
@@ -609,15 +626,16 @@ static void launch_adapters_up(const AdapterCall& q, int units) {
   auto kernel = adapters_up_kernel<TY, SPLIT, MT, RB>;
   if (kSmem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   // units of a warp: up to 8, as few as leave every processor about twelve warps
-  int64_t per_warp = (int64_t)units * q.n_tiles / (12 * (int64_t)processors());
+  const int subs = (q.tile_rows + MT * 16 - 1) / (MT * 16);
+  int64_t per_warp = (int64_t)units * q.n_tiles * subs / (12 * (int64_t)processors());
   per_warp = per_warp < 1 ? 1 : (per_warp > 8 ? 8 : per_warp);
   int chunks = 0;
   for (int p = 0; p < q.parts.n; ++p) {
     const int here = (q.parts.end[p] - (p ? q.parts.end[p - 1] : 0) + 31) / 32;
     chunks += (here + (int)per_warp * kUpWarps - 1) / ((int)per_warp * kUpWarps);
   }
-  launch_kernel(kernel, dim3(q.n_tiles * chunks), dim3(kUpThreads), kSmem, q.stream, (TY*)q.y, q.ldy, q.h, q.b, q.ranks, q.rows, q.tiles, q.tokens, q.listed, q.slots,
-                q.parts, (int)per_warp, chunks, q.rank);
+  launch_kernel(kernel, dim3(q.n_tiles * subs * chunks), dim3(kUpThreads), kSmem, q.stream, (TY*)q.y, q.ldy, q.h, q.b, q.ranks, q.rows, q.tiles, q.tokens, q.listed, q.slots,
+                q.parts, q.tile_rows, subs, (int)per_warp, chunks, q.rank);
 }
 template <typename TY, int SPLIT>
 static int launch_adapters(const AdapterCall& q, int units) {
@@ -646,7 +664,7 @@ static int launch_adapters(const AdapterCall& q, int units) {
   if (q.rank <= 32) {
     few ? launch_adapters_up<TY, SPLIT, 1, 1>(q, units) : launch_adapters_up<TY, SPLIT, 4, 1>(q, units);
   } else if (q.rank <= 64) {
-    few ? launch_adapters_up<TY, SPLIT, 1, 2>(q, units) : launch_adapters_up<TY, SPLIT, 4, 2>(q, units);
+    few ? launch_adapters_up<TY, SPLIT, 1, 2>(q, units) : launch_adapters_up<TY, SPLIT, 2, 2>(q, units);
   } else {
     few ? launch_adapters_up<TY, SPLIT, 1, 0>(q, units) : launch_adapters_up<TY, SPLIT, 4, 0>(q, units);
   }
@@ -697,7 +715,7 @@ extern "C" int roost_adapters_add(void* y, int64_t ldy, const void* x, int64_t l
     ROOST_REQUIRE(h, "adapters_add: the workspace is missing");
     int64_t units = 0;
     for (int p = 0; p < n_parts; ++p) units += (widths[p] + 31) / 32;
-    if (units * n_tiles > 2147483647LL) return fail(ROOST_ERR_UNSUPPORTED, "adapters_add: too many tiles");
+    if (units * 2 * n_tiles > 2147483647LL) return fail(ROOST_ERR_UNSUPPORTED, "adapters_add: too many tiles");
     const AdapterCall q{y,    ldy,     (const __nv_bfloat16*)x, ldx,       (const __nv_bfloat16*)a, (const __nv_bfloat16*)b, (__nv_bfloat16*)h, scales, ranks,
                         rows, tiles, n_tiles,                 tile_rows, listed,                  tokens,                  slots,             rank,   inputs,
                         parts, (cudaStream_t)stream};
