@@ -616,7 +616,8 @@ static void launch_adapters_down(const AdapterCall& q) {
   const size_t sums = (size_t)KG * Cfg::kRowsX * (wide + 31) * sizeof(float), all = (size_t)stages * stage;
   const size_t smem = sums > all ? sums : all;
   auto kernel = adapters_down_kernel<SPLIT, MT, KG, NS, NP, SK>;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  if (smem > 40 * 1024) allow_smem(kernel, 220 * 1024, done);
   launch_kernel_cluster(kernel, dim3(q.n_tiles * ctas), dim3(Cfg::kThreads), smem, q.stream, ctas, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tokens,
                         q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas, stages, stage);
 }
@@ -624,7 +625,8 @@ template <typename TY, int SPLIT, int MT, int RB>
 static void launch_adapters_up(const AdapterCall& q, int units) {
   constexpr int kSmem = UpCfg<TY, MT, RB>::kSmem;
   auto kernel = adapters_up_kernel<TY, SPLIT, MT, RB>;
-  if (kSmem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> done{0};
+  if (kSmem > 40 * 1024) allow_smem(kernel, kSmem, done);
   // units of a warp: up to 8, as few as leave every processor about twelve warps
   const int subs = (q.tile_rows + MT * 16 - 1) / (MT * 16);
   int64_t per_warp = (int64_t)units * q.n_tiles * subs / (12 * (int64_t)processors());

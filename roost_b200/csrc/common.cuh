@@ -92,6 +92,18 @@ inline int processors() {
   return count;
 }
 
+// Allows a kernel `bytes` of dynamic shared memory, beyond the 48 KB that need no word, once a device (`done`: a static of the launching function's, one a
+// kernel; `bytes`: the most that any of its launches takes).
+template <typename Kernel>
+inline void allow_smem(Kernel kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 inline int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {

@@ -707,17 +707,6 @@ int make_map(CUtensorMap* map, const void* base, int rows, int k, int64_t ld, in
   return ROOST_OK;
 }
 
-// Shared memory beyond 48 KB is allowed a kernel once a device.
-template <typename Kernel>
-void allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  done.fetch_or(bit, std::memory_order_relaxed);
-}
-
 struct Operands {
   const void *q, *w;
   const float *q_scale, *w_scale;
@@ -770,7 +759,7 @@ int launch_tile(const Operands& o) {
   if (rc == ROOST_OK) rc = make_map(&mw, o.w, o.n, o.k, o.ldw, BN);
   if (rc != ROOST_OK) return rc;
   auto kernel = gemm_e4m3_tile_kernel<TOut, BN>;
-  allow_smem(kernel, smem, done);
+  allow_smem(kernel, (int)smem, done);
   const int64_t tiles = (int64_t)((o.m + 127) / 128) * ((o.n + BN - 1) / BN);
   const int grid = (int)(tiles < processors() ? tiles : processors());
   launch_kernel(kernel, dim3(grid), dim3(192), smem, o.stream, mq, mw, o.q_scale, o.w_scale, (TOut*)o.out, o.m, o.n, o.k, o.ldo, o.error);
@@ -786,7 +775,7 @@ int launch_pair(const Operands& o) {
   if (rc == ROOST_OK) rc = make_map(&mw, o.w, o.n, o.k, o.ldw, 128);
   if (rc != ROOST_OK) return rc;
   auto kernel = gemm_e4m3_pair_kernel<TOut>;
-  allow_smem(kernel, smem, done);
+  allow_smem(kernel, (int)smem, done);
   const int64_t tiles = (int64_t)((o.m + 255) / 256) * ((o.n + 255) / 256);
   const int pairs = (int)(tiles < processors() / 2 ? tiles : processors() / 2);
   launch_kernel(kernel, dim3(2 * pairs), dim3(192), smem, o.stream, mq, mw, o.q_scale, o.w_scale, (TOut*)o.out, o.m, o.n, o.k, o.ldo, o.error);

@@ -477,7 +477,8 @@ static bool launch_walk(const Source& src, size_t bytes, uint8_t* q, float* scal
   const int by_threads = 1024 / ((threads + 127) / 128 * 128), by_smem = (int)((224 * 1024) / (smem + 2048)), blocks = by_threads < by_smem ? by_threads : by_smem;
   if (!error || blocks < 1) return false;
   auto kernel = rows_e4m3_walk_kernel<KV, Source>;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  if (smem > 40 * 1024) allow_smem(kernel, 220 * 1024, done);
   const int grid = blocks * processors();
   launch_kernel(kernel, dim3(rows < grid ? rows : grid), dim3(threads), smem, stream, src, q, scale, rows, cols, eps, stages, error);
   return true;

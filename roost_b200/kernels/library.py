@@ -17,6 +17,7 @@ from . import build
 
 ABI_VERSION = 18
 F32, BF16 = 0, 1
+E4M3 = torch.float8_e4m3fn
 GATE_FUNCTIONS = {"silu": 0, "gelu_tanh": 1, "clamped_swish": 2}   # the codes of csrc/roost_kernels.h
 
 
@@ -48,6 +49,11 @@ def _stream():
     return _raw_stream(torch.cuda.current_device())
 
 
+def _stream_of(device: int):
+    """The same of a device that is known to be the current one."""
+    return _stream() if _raw_stream is None else _raw_stream(device)
+
+
 def _need(t: torch.Tensor, name: str, dtype=None):
     if not t.is_cuda:
         raise KernelError(f"{name} is not on a CUDA device")
@@ -57,15 +63,19 @@ def _need(t: torch.Tensor, name: str, dtype=None):
         raise KernelError(f"{name} has dtype {t.dtype}; expected {dtype}")
 
 
-def _need_here(**tensors):
-    """Every tensor given (None: left out) lies on the current device, whose current stream the call goes to."""
-    for name, t in tensors.items():
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _need_here(what: str, *tensors) -> int:
+    """The device of the tensors (None: left out), which is the current one: the call goes to its current stream."""
+    for t in tensors:
         if t is not None and not t.is_cuda:
-            raise KernelError(f"{name} is not on a CUDA device")
-    here = torch.cuda.current_device()
-    for name, t in tensors.items():
-        if t is not None and t.device.index != here:
-            raise KernelError(f"{name} is on {t.device}; the call goes to the current device, cuda:{here}")
+            raise KernelError(f"{what}: a tensor is on {t.device}, not on a CUDA device")
+    here = _current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise KernelError(f"{what}: a tensor is on {t.device}; the call goes to the current device, cuda:{here}")
+    return here
 
 
 def _need_rows(t: torch.Tensor, name: str, dtype=None):
@@ -335,6 +345,7 @@ class KernelLibrary:
         self.decode_chunk = 512  # keys per work item of the split decode attention (see decode_chunk_for)
         self.decode_cluster = True  # split rows merged by thread-block clusters where they fit (see decode_cluster_for)
         self._decode_ctas = 0
+        self._adapter_workspace = {}    # (listed, parts, rank, dtypes) -> bytes
         self.launches = 0  # kernels launched through this handle (a host-side count of entry-point calls that launch)
         self.library_launches = 0  # products handed to cuBLAS through torch beside them (counted where they are called)
 
@@ -442,41 +453,45 @@ class KernelLibrary:
         return out
 
     # ---- rows in 8 bits. A row v stands as q (e4m3) times scale (float32), scale = max(max |v| / 448, 2^-126) and q nearest to v / scale. A row
-    # that holds an infinity or a NaN makes its row of a product NaN.
-    @staticmethod
-    def _e4m3_rows(shape, device):
-        return torch.empty(shape, dtype=torch.float8_e4m3fn, device=device), torch.empty(shape[:-1], dtype=torch.float32, device=device)
-
+    # that holds an infinity or a NaN makes its row of a product NaN. (These run a hundred times a decode step, so they form no more than they need.)
     def quantise_e4m3(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """(q, scale) of the rows of x [T, W], which may lie apart: activations ahead of ``gemm_e4m3``, or a weight's rows."""
-        _need_here(x=x); _need_rows(x, "x")
+        here = _need_here("quantise_e4m3", x)
+        _need_rows(x, "x")
         T, W = x.shape
-        q, scale = self._e4m3_rows((T, W), x.device)
-        self._call("roost_quantise_e4m3", _ptr(x), x.stride(0) if T > 1 else W, _ptr(q), _ptr(scale), T, W, dtype_code(x.dtype), _stream())
+        q = torch.empty_like(x, dtype=E4M3) if x.is_contiguous() else x.new_empty((T, W), dtype=E4M3)
+        scale = x.new_empty(T, dtype=torch.float32)
+        self._call("roost_quantise_e4m3", x.data_ptr(), x.stride(0) if T > 1 else W, q.data_ptr(), scale.data_ptr(), T, W, dtype_code(x.dtype), _stream_of(here))
         return q, scale
 
     def silu_mul_e4m3(self, x: torch.Tensor, block: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
         """(q, scale) of silu(gate) * up, which is not rounded before; x and ``block`` as ``silu_mul``."""
-        _need_here(x=x); _need(x, "x")
+        here = _need_here("silu_mul_e4m3", x)
+        _need(x, "x")
         if x.dim() != 2 or x.shape[1] % 2:
             raise KernelError(f"silu_mul_e4m3: x is {tuple(x.shape)}; expected rows of gate and up values")
         T, inter = x.shape[0], x.shape[1] // 2
-        q, scale = self._e4m3_rows((T, inter), x.device)
-        self._call("roost_silu_mul_e4m3", _ptr(x), _ptr(q), _ptr(scale), T, inter, block, dtype_code(x.dtype), _stream())
+        q, scale = x.new_empty((T, inter), dtype=E4M3), x.new_empty(T, dtype=torch.float32)
+        self._call("roost_silu_mul_e4m3", x.data_ptr(), q.data_ptr(), scale.data_ptr(), T, inter, block, dtype_code(x.dtype), _stream_of(here))
         return q, scale
 
     def _rms_norm_e4m3(self, x, residual, w, eps, rows, keep):
-        _need_here(x=x, residual=residual, w=w, rows=rows); _need(x, "x"); _need(w, "w")
+        here = _need_here("rms_norm_e4m3", x, residual, w, rows)
+        _need(x, "x"); _need(w, "w")
         H = x.shape[-1]
         if w.numel() != H:
             raise KernelError(f"rms_norm_e4m3: weight has {w.numel()} elements for rows of {H}")
-        if rows is not None:
+        if rows is None:
+            q = torch.empty_like(x, dtype=E4M3)
+            scale = x.new_empty(x.shape[0] if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
+            kept = torch.empty_like(x) if keep else None
+        else:
             _need(rows, "rows", torch.int32)
-        shape = tuple(x.shape) if rows is None else (rows.numel(), H)
-        q, scale = self._e4m3_rows(shape, x.device)
-        kept = torch.empty(shape, dtype=x.dtype, device=x.device) if keep else None
-        self._call("roost_rms_norm_e4m3", _ptr(x), _ptr(residual), _ptr(w), _ptr(q), _ptr(scale), _ptr(kept), _ptr(rows), scale.numel(), H, eps,
-                   dtype_code(x.dtype), dtype_code(x.dtype if residual is None else residual.dtype), dtype_code(w.dtype), _stream())
+            q, scale = x.new_empty((rows.numel(), H), dtype=E4M3), x.new_empty(rows.numel(), dtype=torch.float32)
+            kept = x.new_empty((rows.numel(), H)) if keep else None
+        code = dtype_code(x.dtype)
+        self._call("roost_rms_norm_e4m3", x.data_ptr(), _ptr(residual), w.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(kept), _ptr(rows), scale.numel(), H, eps,
+                   code, code if residual is None else dtype_code(residual.dtype), dtype_code(w.dtype), _stream_of(here))
         return (q, scale, kept) if keep else (q, scale)
 
     def rms_norm_e4m3(self, x: torch.Tensor, w: torch.Tensor, eps: float, rows: torch.Tensor | None = None, keep: bool = False):
@@ -494,15 +509,16 @@ class KernelLibrary:
 
     def gemm_e4m3(self, q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k] for rows in 8 bits on either side (``quantise_e4m3`` and its like), 32-bit sums."""
-        _need_here(q=q, q_scale=q_scale, w=w, w_scale=w_scale)
-        _need_rows(q, "q", torch.float8_e4m3fn); _need_rows(w, "w", torch.float8_e4m3fn)
+        here = _need_here("gemm_e4m3", q, q_scale, w, w_scale)
+        _need_rows(q, "q", E4M3); _need_rows(w, "w", E4M3)
         _need(q_scale, "q_scale", torch.float32); _need(w_scale, "w_scale", torch.float32)
         (M, K), (N, K2) = q.shape, w.shape
         if K != K2 or q_scale.numel() != M or w_scale.numel() != N:
             raise KernelError(f"gemm_e4m3: q {tuple(q.shape)}, w {tuple(w.shape)} and scales of {q_scale.numel()} and {w_scale.numel()} rows do not agree")
-        out = torch.empty((M, N), dtype=out_dtype, device=q.device)
-        self._call("roost_gemm_e4m3", _ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), _ptr(out), M, N, K, q.stride(0) if M > 1 else K,
-                   w.stride(0) if N > 1 else K, N, dtype_code(out_dtype), _stream())
+        code = dtype_code(out_dtype)
+        out = q_scale.new_empty((M, N), dtype=out_dtype)
+        self._call("roost_gemm_e4m3", q.data_ptr(), q_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), out.data_ptr(), M, N, K, q.stride(0) if M > 1 else K,
+                   w.stride(0) if N > 1 else K, N, code, _stream_of(here))
         return out
 
     # ---- adapters
@@ -519,7 +535,7 @@ class KernelLibrary:
         the shared projection made of x, rows [T, N] that may lie apart, in x's type (or float32 beside bfloat16). ``widths``: the parts of the
         projection's outputs (queries, keys and values, say), each with an adapter of its own; None: one part. a [slots, parts, rank, K] and b
         [slots, N, rank] in x's type, scale float32 [slots]; ``ranks`` int32 [slots]: how many of the rank's rows a slot uses (None: all)."""
-        _need_here(y=y, x=x, a=a, b=b, scale=scale, ranks=ranks, rows=plan.rows, tiles=plan.tiles)
+        here = _need_here("adapters_add_", y, x, a, b, scale, ranks, plan.rows, plan.tiles)
         _need_rows(y, "y"); _need_rows(x, "x"); _need(a, "a", x.dtype); _need(b, "b", x.dtype); _need(scale, "scale", torch.float32)
         _need(plan.rows, "the plan's rows", torch.int32); _need(plan.tiles, "the plan's tiles", torch.int32)
         (T, N), K = y.shape, x.shape[1]
@@ -534,11 +550,13 @@ class KernelLibrary:
             if ranks.numel() != S:
                 raise KernelError(f"adapters_add_: {ranks.numel()} ranks for {S} slots")
         codes, listed = (dtype_code(x.dtype), dtype_code(y.dtype)), plan.rows.numel()
-        need = self._lib.roost_adapters_workspace_bytes(listed, P, R, *codes)
-        h = torch.empty(need, dtype=torch.uint8, device=y.device) if need else None
-        self._call("roost_adapters_add", _ptr(y), y.stride(0) if T > 1 else N, _ptr(x), x.stride(0) if T > 1 else K, _ptr(a), _ptr(b), _ptr(h), _ptr(scale),
-                   _ptr(ranks), _ptr(plan.rows), _ptr(plan.tiles), plan.tiles.shape[0], plan.tile_rows, listed, T, S, P, (c_int * P)(*widths), R, K, *codes,
-                   _stream(), launches=2 if need else 1)
+        need = self._adapter_workspace.get((listed, P, R, codes))
+        if need is None:
+            need = self._adapter_workspace[(listed, P, R, codes)] = self._lib.roost_adapters_workspace_bytes(listed, P, R, *codes)
+        h = x.new_empty(need, dtype=torch.uint8) if need else None
+        self._call("roost_adapters_add", y.data_ptr(), y.stride(0) if T > 1 else N, x.data_ptr(), x.stride(0) if T > 1 else K, a.data_ptr(), b.data_ptr(), _ptr(h),
+                   scale.data_ptr(), _ptr(ranks), plan.rows.data_ptr(), plan.tiles.data_ptr(), plan.tiles.shape[0], plan.tile_rows, listed, T, S, P,
+                   (c_int * P)(*widths), R, K, *codes, _stream_of(here), launches=2 if need else 1)
         return y
 
     def rope_table(self, positions: torch.Tensor, inv_freq: torch.Tensor) -> torch.Tensor:
