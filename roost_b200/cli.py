@@ -22,7 +22,7 @@ and exits with 2.
                                                       unless --seed is given), so that its pinned tokens can be reproduced
     roost replay --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N      (bin/trace_run)
     roost doctor [--model DIR] [--kernels DIR] [--no-gpu] [--min-free-memory-gib N]
-  engine options: [--dtype bfloat16|float32] [--device N] [--kernels DIR] [--page-size N] [--attention-blocks N]
+  engine options: [--dtype bfloat16|float32] [--weights stored|e4m3] [--device N] [--kernels DIR] [--page-size N] [--attention-blocks N]
                   [--kv-fraction F] [--max-tokens N] [--max-sequences N] [--max-chunk-tokens N]
 """
 from __future__ import annotations
@@ -33,7 +33,7 @@ import sys
 
 USAGE = __doc__.split("\n\n", 2)[2]
 
-_ENGINE_VALUED = {"--dtype", "--device", "--kernels", "--page-size", "--attention-blocks", "--kv-fraction", "--max-tokens",
+_ENGINE_VALUED = {"--dtype", "--weights", "--device", "--kernels", "--page-size", "--attention-blocks", "--kv-fraction", "--max-tokens",
                   "--max-sequences", "--max-chunk-tokens"}
 _COMMANDS = {
     "generate": (_ENGINE_VALUED | {"--model", "--prompt-ids", "--prompt-file", "--max-output-tokens", "--temperature", "--top-p",
@@ -110,6 +110,15 @@ def _need(opts, key):
     return opts[key]
 
 
+def _weights(opts, dtype: str) -> str:
+    weights = opts.get("--weights", "stored")
+    if weights not in ("stored", "e4m3"):
+        raise UsageError("--weights is stored or e4m3")
+    if weights == "e4m3" and dtype != "bfloat16":
+        raise UsageError("--weights e4m3 needs --dtype bfloat16")
+    return weights
+
+
 def _kv_fraction(opts) -> float:
     """--kv-fraction: the share of the device memory free after the weights that the cache pools take when
     --attention-blocks does not size them."""
@@ -160,7 +169,7 @@ def cmd_generate(opts) -> int:
     # every option is read before anything is loaded, so a bad value is a usage error whatever the model is
     engine_opts = dict(page_size=_int(opts, "--page-size", 16), attention_blocks=_int(opts, "--attention-blocks"), kv_fraction=_kv_fraction(opts),
                        max_sequences=_int(opts, "--max-sequences", 64), max_tokens=_int(opts, "--max-tokens", 2048),
-                       max_chunk_tokens=_int(opts, "--max-chunk-tokens"))
+                       max_chunk_tokens=_int(opts, "--max-chunk-tokens"), weights=_weights(opts, dtype))
     gen_opts = dict(max_output_tokens=_int(opts, "--max-output-tokens", 16), temperature=_float(opts, "--temperature"),
                     top_p=_float(opts, "--top-p"), top_k=_int(opts, "--top-k"), min_p=_float(opts, "--min-p"),
                     seed=_int(opts, "--seed"), stop_token_ids=tuple(_ids(opts.get("--stop-ids", ""), "--stop-ids")),
@@ -208,7 +217,7 @@ def cmd_chat(opts, lines=None, out=None) -> int:
         raise UsageError("--dtype is bfloat16 or float32")
     engine_opts = dict(page_size=_int(opts, "--page-size", 16), attention_blocks=_int(opts, "--attention-blocks"), kv_fraction=_kv_fraction(opts),
                        max_sequences=_int(opts, "--max-sequences", 1), max_tokens=_int(opts, "--max-tokens", 2048),
-                       max_chunk_tokens=_int(opts, "--max-chunk-tokens"))
+                       max_chunk_tokens=_int(opts, "--max-chunk-tokens"), weights=_weights(opts, dtype))
     gen_opts = dict(max_output_tokens=_int(opts, "--max-output-tokens", 256), temperature=_float(opts, "--temperature"),
                     top_p=_float(opts, "--top-p"), top_k=_int(opts, "--top-k"), min_p=_float(opts, "--min-p"),
                     seed=_int(opts, "--seed"), stop_token_ids=tuple(_ids(opts.get("--stop-ids", ""), "--stop-ids")),
@@ -305,7 +314,7 @@ def cmd_bench(opts) -> int:
         raise UsageError("--batch, --prompt-tokens and --new-tokens must be positive")
     engine_opts = dict(page_size=_int(opts, "--page-size", 16), attention_blocks=_int(opts, "--attention-blocks"), kv_fraction=_kv_fraction(opts),
                        max_sequences=_int(opts, "--max-sequences", max(batch, 1)), max_tokens=_int(opts, "--max-tokens", 2048),
-                       max_chunk_tokens=_int(opts, "--max-chunk-tokens"))
+                       max_chunk_tokens=_int(opts, "--max-chunk-tokens"), weights=_weights(opts, dtype))
     seed = _int(opts, "--seed", 0)
     _apply_common(opts)
     import torch

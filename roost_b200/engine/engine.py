@@ -94,8 +94,9 @@ class Completion:
 class RoostEngine:
     def __init__(self, model, *, dtype: str | torch.dtype = "bfloat16", device: str = "cuda", page_size: int = 16,
                  attention_blocks: int | None = None, kv_fraction: float = 0.9, max_sequences: int = 64, max_tokens: int = 2048,
-                 max_chunk_tokens: int | None = None, seed: int | None = None, chain_steps: bool = True):
-        """``model``: a folder with config.json and model.safetensors, or a built ``Model``. ``attention_blocks``:
+                 max_chunk_tokens: int | None = None, seed: int | None = None, chain_steps: bool = True, weights: str = "stored"):
+        """``model``: a folder with config.json and model.safetensors, or a built ``Model``. ``weights``: "stored", or "e4m3" for the layers'
+        projections in 8 bits with a scale an output row (``load_model``; a built ``Model`` has its form already). ``attention_blocks``:
         pages in each paged pool (else ``kv_fraction`` of the free device memory); ``max_tokens`` and
         ``max_sequences``: the largest token and row count of a step (the reference's worker flags of the same
         names, src/Starlings.Roost.WorkerHost/WorkerArguments.cs:51-58). ``chain_steps``: while every live request
@@ -105,7 +106,9 @@ class RoostEngine:
         not seen, which is this engine's own addition); the tokens are the same with it and without."""
         if isinstance(dtype, str):
             dtype = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}[dtype]
-        self.model: Model = model if isinstance(model, Model) else load_model(model, dtype, device)
+        if isinstance(model, Model) and weights != "stored" and model.rt.weights != weights:
+            raise ValueError(f"the model was built with weights {model.rt.weights!r}, not {weights!r}")
+        self.model: Model = model if isinstance(model, Model) else load_model(model, dtype, device, weights=weights)
         self.executor = StepExecutor(self.model, page_size=page_size, num_pages=attention_blocks, max_requests=max_sequences,
                                      kv_fraction=kv_fraction)
         spec = self.model.spec

@@ -14,7 +14,7 @@ import torch
 from ..config.reader import ConfigReader
 from ..config.spec import ModelSpec
 from ..parts.base import BLOCKS, EMBEDDINGS, HEADS, NORMS, ParamDecl, Runtime
-from ..parts.linear import Linear
+from ..parts.linear import E4m3Linear, Linear
 from .. import registry
 from ..weights import loader as weight_loader
 
@@ -45,6 +45,11 @@ class Model:
         # what each run keeps between steps (None: nothing, or another run's cache)
         self.cache_needs = []
         self.embedding_need = self.embedding.cache_need()
+        if runtime.e4m3:
+            for i, b in enumerate(self.blocks):
+                for name, part in {"block": b, **b.sub_parts()}.items():
+                    if not getattr(part, "serves_e4m3", False):
+                        raise ValueError(f"weights in e4m3: layer {i}'s {name} ({type(part).__name__}) has no form for them")
         for n, e in enumerate(spec.schedule):
             need = self.blocks[e.block].mixer.cache_need()
             if e.reads_cache_of is not None:
@@ -126,6 +131,9 @@ class Model:
                     add(v)
                 elif isinstance(v, Linear):
                     add(v.weight)
+                elif isinstance(v, E4m3Linear):
+                    add(v.weight)
+                    add(v.scale)
                 elif hasattr(v, "weight") and isinstance(getattr(v, "weight"), torch.Tensor):
                     add(v.weight)
         add(self.final_norm.weight)
@@ -169,15 +177,16 @@ def read_model_config(model_dir):
     return arch, cfg, reader
 
 
-def load_model(model_dir, dtype: torch.dtype, device="cuda", kernels=None) -> Model:
-    """Builds the model config.json names and loads model.safetensors into it."""
+def load_model(model_dir, dtype: torch.dtype, device="cuda", kernels=None, weights: str = "stored") -> Model:
+    """Builds the model config.json names and loads model.safetensors into it. ``weights`` "e4m3": the layers' projections in 8 bits (bfloat16
+    models of pre_norm layers of paged attention and gated feed-forwards; the embedding and the head stay as they are)."""
     from ..kernels import library
     arch, cfg, _ = read_model_config(model_dir)
     tied = getattr(cfg, "tie_word_embeddings", None)
     if tied is None:
         tied = not weight_loader.checkpoint_has(model_dir, "lm_head.weight")
     spec = arch.to_spec(cfg, tied)
-    runtime = Runtime(dtype, device, kernels if kernels is not None else library.load())
+    runtime = Runtime(dtype, device, kernels if kernels is not None else library.load(), weights)
     model = Model(spec, runtime)
     decls = parameter_declarations(spec)
     allow = (("lm_head.weight",) if spec.tie_embeddings else ()) + tuple(spec.ignorable_tensors)

@@ -16,13 +16,15 @@ import numpy as np
 from ..config.spec import AttentionSpec
 from .attention_work import AttentionPlan, attention_caps, attention_work
 from .base import NORMS, POSITIONS, CacheNeed, Mixer, ParamDecl, Runtime, register_mixer
-from .linear import Linear
+from .linear import projection
 from .positions import require_plain_amplitude
 
 SHORT_ROW_TOKENS = 16   # rows of at most this many tokens may go to the split decode kernel
 
 
 class PagedAttention(Mixer):
+    serves_e4m3 = True
+
     def __init__(self, spec: AttentionSpec, runtime: Runtime):
         s = spec
         if min(s.hidden, s.num_heads, s.num_kv_heads, s.head_dim) <= 0:
@@ -41,9 +43,9 @@ class PagedAttention(Mixer):
         self.rt = runtime
         self.q_width = s.num_heads * s.head_dim
         self.kv_width = s.num_kv_heads * s.head_dim
-        self.qkv = Linear(runtime, self.q_width + 2 * self.kv_width, s.hidden)
-        self.out = Linear(runtime, s.hidden, self.q_width)
-        self.q_only: Linear | None = None   # the q rows of qkv, for runs that read another run's cache
+        self.qkv = projection(runtime, self.q_width + 2 * self.kv_width, s.hidden)
+        self.out = projection(runtime, s.hidden, self.q_width)
+        self.q_only = None   # the q rows of qkv, for runs that read another run's cache
         self.q_norm = self.k_norm = None
         if s.qk_norm is not None:
             if s.qk_norm.size != s.head_dim:
@@ -94,8 +96,7 @@ class PagedAttention(Mixer):
                                      page_size=cache.page_size, write_kv=True)
         else:
             if self.q_only is None:
-                self.q_only = Linear(self.rt, self.q_width, s.hidden)
-                self.q_only.load(self.qkv.weight[: self.q_width])
+                self.q_only = self.qkv.first_rows(self.q_width)
             q = k.qk_norm_rope_cache(self.q_only(x), s.num_heads, s.num_kv_heads, s.head_dim, q_w=qw, k_w=kw, eps=eps,
                                      inv_freq=inv_freq, rotary_dim=rotary_dim, positions=batch.positions, write_kv=False, cos_sin=table)
         o = self.attend(q, batch, cache, tables)

@@ -53,13 +53,23 @@ class CacheNeed:
     keep_first: int = 0
 
 
+WEIGHT_FORMS = ("stored", "e4m3")
+
+
 class Runtime:
     """What every part is built with: the compute dtype of activations (and of the cache), the device, and
     the kernel library handle (None only for declaring parameters on a machine without a GPU)."""
 
-    def __init__(self, dtype: torch.dtype, device, kernels=None):
+    def __init__(self, dtype: torch.dtype, device, kernels=None, weights: str = "stored"):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype {dtype} is not float32 or bfloat16")
+        if weights not in WEIGHT_FORMS:
+            raise ValueError(f"weights {weights!r} is not one of {', '.join(WEIGHT_FORMS)}")
+        if weights == "e4m3" and dtype != torch.bfloat16:
+            raise ValueError("weights in e4m3 are multiplied with rows in e4m3: the compute dtype is bfloat16")
+        # "e4m3": the layers' projections hold their weights in 8 bits with a scale an output row and take rows in 8 bits
+        # (parts that say ``serves_e4m3``)
+        self.weights = weights
         self.dtype = dtype
         self.device = torch.device(device)
         self.kernels = kernels
@@ -72,6 +82,10 @@ class Runtime:
     def full_precision(self) -> bool:
         return self.dtype == torch.float32
 
+    @property
+    def e4m3(self) -> bool:
+        return self.weights == "e4m3"
+
 
 class Part:
     spec = None
@@ -79,6 +93,9 @@ class Part:
     # data (routing written in Python, say): a model with such a part runs its steps eagerly instead of
     # replaying captured CUDA graphs. A class that does not derive from Part may set the attribute all the same.
     capturable = True
+    # True for a part that runs with ``Runtime.weights`` "e4m3": its projections are ``projection``s and take the rows in 8 bits of
+    # the norm in front of them
+    serves_e4m3 = False
 
     @classmethod
     def parameters(cls, spec) -> dict[str, ParamDecl]:

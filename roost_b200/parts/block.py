@@ -11,6 +11,8 @@ from .base import CONNECTIONS, FEED_FORWARDS, MIXERS, NORMS, TOKEN_INPUTS, Block
 
 
 class PreNormBlock(Block):
+    serves_e4m3 = True
+
     def __init__(self, spec: BlockSpec, runtime: Runtime):
         self.spec = spec
         self.rt = runtime
@@ -31,6 +33,15 @@ class PreNormBlock(Block):
     def __call__(self, h, residual, batch, cache, write_cache: bool = True):
         """``h`` is the previous branch output (or the embedding), ``residual`` the stream before it was added
         (None at the first block). Returns the feed-forward's output and the stream it is still to be added to."""
+        if self.rt.e4m3:      # the norms hand their rows over in 8 bits
+            if residual is None:
+                residual = h
+                x = self.input_norm.rows_e4m3(h)
+            else:
+                x, residual = self.input_norm.add_norm_e4m3(h, residual)
+            a = self.mixer(x, batch, cache, write_cache)
+            y, residual = self.post_mixer_norm.add_norm_e4m3(a, residual)
+            return self.feed_forward(y, batch), residual
         if residual is None:
             residual = h
             x = self.input_norm(h)

@@ -10,6 +10,8 @@ wherever they serve, "library" forces cuBLAS.
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from .base import Runtime
@@ -77,6 +79,51 @@ class Linear:
             k.library_launches += 1
             return torch.mm(x, self.weight.t(), out_dtype=torch.float32)
         return k.gemm_simt(x, self.weight, torch.float32)
+
+
+    def first_rows(self, n: int) -> "Linear":
+        """A projection onto the first ``n`` outputs, over the same weight."""
+        part = Linear(self.rt, n, self.in_features)
+        part.load(self.weight[:n])
+        return part
+
+
+class E4m3Rows(NamedTuple):
+    """Rows in 8 bits: row t stands for q[t] * scale[t] (``KernelLibrary.quantise_e4m3``)."""
+    q: torch.Tensor
+    scale: torch.Tensor
+
+
+class E4m3Linear:
+    """y = x W^T with W in 8 bits, a scale an output row, quantised once at load from the weight as it is computed with otherwise. x: rows in 8
+    bits, as the norms and gates of ``Runtime.weights`` "e4m3" hand them over, or plain rows, which are quantised first."""
+
+    def __init__(self, runtime: Runtime, out_features: int, in_features: int):
+        self.rt = runtime
+        self.out_features = out_features
+        self.in_features = in_features
+        self.weight: torch.Tensor | None = None      # e4m3 [out, in]
+        self.scale: torch.Tensor | None = None       # float32 [out]
+
+    def load(self, weight: torch.Tensor) -> None:
+        if tuple(weight.shape) != (self.out_features, self.in_features):
+            raise ValueError(f"linear: weight is {tuple(weight.shape)}; expected {(self.out_features, self.in_features)}")
+        self.weight, self.scale = self.rt.kernels.quantise_e4m3(weight.to(self.rt.dtype).contiguous())
+
+    def __call__(self, x, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+        k = self.rt.kernels
+        q, scale = x if isinstance(x, E4m3Rows) else k.quantise_e4m3(x)
+        return k.gemm_e4m3(q, scale, self.weight, self.scale, out_dtype or self.rt.dtype)
+
+    def first_rows(self, n: int) -> "E4m3Linear":
+        part = E4m3Linear(self.rt, n, self.in_features)
+        part.weight, part.scale = self.weight[:n], self.scale[:n]
+        return part
+
+
+def projection(runtime: Runtime, out_features: int, in_features: int):
+    """A layer's projection without a bias, in the form ``Runtime.weights`` asks for."""
+    return (E4m3Linear if runtime.e4m3 else Linear)(runtime, out_features, in_features)
 
 
 def batched_linear_f32(rt: Runtime, a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:

@@ -9,13 +9,15 @@ import math
 
 from ..config.spec import DenseMlpSpec, GatedMlpSpec
 from .base import FeedForward, ParamDecl, Runtime, register_feed_forward
-from .linear import Linear
+from .linear import E4m3Rows, Linear, projection
 
 
 GATE_FUNCTIONS = ("silu", "gelu_tanh", "clamped_swish")
 
 
 class GatedMlp(FeedForward):
+    serves_e4m3 = True
+
     def __init__(self, spec: GatedMlpSpec, runtime: Runtime):
         if spec.hidden <= 0 or spec.intermediate <= 0:
             raise ValueError("gated_mlp: hidden and intermediate must be positive")
@@ -25,14 +27,16 @@ class GatedMlp(FeedForward):
             raise ValueError("gated_mlp: the clamped swish needs a positive limit")
         self.spec = spec
         self.rt = runtime
-        self.gate_up = Linear(runtime, 2 * spec.intermediate, spec.hidden)
-        self.down = Linear(runtime, spec.hidden, spec.intermediate)
+        if runtime.e4m3 and spec.activation != "silu":
+            raise ValueError(f"gated_mlp: weights in e4m3 serve the activation 'silu', not '{spec.activation}'")
+        self.gate_up = projection(runtime, 2 * spec.intermediate, spec.hidden)
+        self.down = projection(runtime, spec.hidden, spec.intermediate)
         # In bfloat16 with an intermediate size that is a multiple of 128 the gate and up rows are stored interleaved in
         # blocks of 128, the layout in which the tensor-core product applies SiLU(gate) * up to its accumulator, so that
         # for many rows of x the [T, 2I] product never goes to memory; few rows keep the library product and the
         # SiLU kernel, which reads the same layout.
         k = runtime.kernels
-        self.interleave = 128 if (not runtime.full_precision and spec.intermediate % 128 == 0 and spec.hidden % 8 == 0
+        self.interleave = 128 if (not runtime.full_precision and not runtime.e4m3 and spec.intermediate % 128 == 0 and spec.hidden % 8 == 0
                                   and spec.activation == "silu" and hasattr(k, "gemm_tcgen05_swiglu")) else 0
         self.fused_min_rows = 256   # below this the 128-row tiles are mostly empty and the library product is faster
         # ... and so it is while the product is small: measured on a B200, the library product followed by the SiLU kernel
@@ -67,6 +71,8 @@ class GatedMlp(FeedForward):
 
     def __call__(self, x, batch=None):
         k = self.rt.kernels
+        if self.rt.e4m3:
+            return self.down(E4m3Rows(*k.silu_mul_e4m3(self.gate_up(x))))
         if self.spec.activation != "silu":
             return self.down(k.gated_act_mul(self.gate_up(x), self.spec.activation, float(self.spec.limit)))
         if (self.interleave and x.shape[0] >= self.fused_min_rows and x.is_contiguous()

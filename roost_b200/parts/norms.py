@@ -7,9 +7,12 @@ import torch
 
 from ..config.spec import NormSpec
 from .base import Norm, ParamDecl, Runtime, register_norm
+from .linear import E4m3Rows
 
 
 class RmsNorm(Norm):
+    serves_e4m3 = True
+
     def __init__(self, spec: NormSpec, runtime: Runtime):
         if spec.size <= 0 or spec.eps <= 0:
             raise ValueError(f"rms_norm: size {spec.size} and eps {spec.eps} must be positive")
@@ -33,6 +36,14 @@ class RmsNorm(Norm):
         """Returns (norm(residual + x), residual + x); without ``rows`` the sum replaces ``residual`` in place."""
         out = self.rt.kernels.add_rms_norm(x, residual, self.weight, self.spec.eps, rows)
         return out, residual
+
+    def rows_e4m3(self, x: torch.Tensor) -> E4m3Rows:
+        """The norm's rows in 8 bits, for a projection with weights in 8 bits."""
+        return E4m3Rows(*self.rt.kernels.rms_norm_e4m3(x, self.weight, self.spec.eps))
+
+    def add_norm_e4m3(self, x: torch.Tensor, residual: torch.Tensor):
+        """``add_norm`` with the norm's rows in 8 bits."""
+        return E4m3Rows(*self.rt.kernels.add_rms_norm_e4m3(x, residual, self.weight, self.spec.eps)), residual
 
 
 class LayerNorm(Norm):

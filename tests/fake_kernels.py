@@ -32,6 +32,31 @@ class FakeKernels:
             residual.copy_(s)
         return self.rms_norm(s, w, eps, rows)
 
+    @staticmethod
+    def _rows_e4m3(v):
+        scale = (v.abs().amax(-1) / 448.0).clamp_min(2.0 ** -126)
+        return (v / scale[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn), scale
+
+    def quantise_e4m3(self, x):
+        return self._rows_e4m3(x.float())
+
+    def rms_norm_e4m3(self, x, w, eps, rows=None, keep=False):
+        v = self.rms_norm(x.float(), w, eps, rows)
+        return (*self._rows_e4m3(v), v.to(x.dtype)) if keep else self._rows_e4m3(v)
+
+    def add_rms_norm_e4m3(self, x, residual, w, eps, rows=None, keep=False):
+        s = (x.float() + residual.float()).to(residual.dtype)
+        if rows is None:
+            residual.copy_(s)
+        v = self.rms_norm(s.float(), w, eps, rows)
+        return (*self._rows_e4m3(v), v.to(x.dtype)) if keep else self._rows_e4m3(v)
+
+    def silu_mul_e4m3(self, x, block=0):
+        return self._rows_e4m3(self.silu_mul(x.float(), block))
+
+    def gemm_e4m3(self, q, q_scale, w, w_scale, out_dtype=torch.bfloat16):
+        return (q.float() @ w.float().T * w_scale * q_scale[:, None]).to(out_dtype)
+
     def silu_mul(self, x, block=0):
         i = x.shape[1] // 2
         if block:
