@@ -396,7 +396,10 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : 3)
     chunk -= here;
     begin = parts.end[p++];
   }
-  const int first = (chunk * kUpWarps + warp) * per_warp, mine = at.rank == 0 ? 0 : min(per_warp, units - first), end = parts.end[p];
+  // the block's warps take neighbouring units, so that what is on its way at a time are long pieces of y's rows
+  constexpr int kStep = 32 * kUpWarps;
+  const int first = chunk * kUpWarps * per_warp + warp, end = parts.end[p];
+  const int mine = at.rank == 0 ? 0 : min(per_warp, (units - first + kUpWarps - 1) / kUpWarps);
   if (mine <= 0) {
     pdl_wait();
     return;
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : 3)
         adapter_queue16(lane_queue + (uint32_t)((ask_b_at * Cfg::kPieces + Cfg::kY + 4 * v + t) * 512), in ? b + (int64_t)col * R + 32 * v : b, in);
       }
     }
-    ask_b_n += 32;
+    ask_b_n += kStep;
     next(ask_b_at);
   };
   TY* yr[2 * MT];
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : 3)
       for (int v = 0; v < kVecs; ++v)
         adapter_queue16(lane_queue + (uint32_t)((ask_y_at * Cfg::kPieces + i * kVecs + v) * 512), in ? yr[i] + ask_y_n + v * (8 / kVecs) : y, in);
     }
-    ask_y_n += 32;
+    ask_y_n += kStep;
     next(ask_y_at);
     copy_commit();
   };
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(kUpThreads, MT == 1 ? 4 : 3)
     }
   }
 #pragma unroll 1
-  for (int u = 0; u < mine; ++u, n0 += 32) {
+  for (int u = 0; u < mine; ++u, n0 += kStep) {
     if (u + kUpDepth - 1 < mine) {
       ask_b();
       ask_y();
@@ -622,25 +625,35 @@ static void launch_adapters_down(const AdapterCall& q) {
                         q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas, stages, stage);
 }
 template <typename TY, int SPLIT, int MT, int RB>
-static void launch_adapters_up(const AdapterCall& q, int units) {
+static void launch_adapters_up(const AdapterCall& q) {
   constexpr int kSmem = UpCfg<TY, MT, RB>::kSmem;
   auto kernel = adapters_up_kernel<TY, SPLIT, MT, RB>;
   static std::atomic<uint64_t> done{0};
   if (kSmem > 40 * 1024) allow_smem(kernel, kSmem, done);
-  // units of a warp: up to 8, as few as leave every processor about twelve warps
-  const int subs = (q.tile_rows + MT * 16 - 1) / (MT * 16);
-  int64_t per_warp = (int64_t)units * q.n_tiles * subs / (12 * (int64_t)processors());
-  per_warp = per_warp < 1 ? 1 : (per_warp > 8 ? 8 : per_warp);
-  int chunks = 0;
-  for (int p = 0; p < q.parts.n; ++p) {
-    const int here = (q.parts.end[p] - (p ? q.parts.end[p - 1] : 0) + 31) / 32;
-    chunks += (here + (int)per_warp * kUpWarps - 1) / ((int)per_warp * kUpWarps);
+  // Units of a warp: those with which the blocks' turns take the least time, a block's start counted as two units (prompts of 4,001 tokens beside 2 x 12,288
+  // outputs: 8 units in 3.4 turns 92 us, 14 in 2.0 the same; of 4,000 with rank 128 beside 4,096 138 and 104).
+  const int subs = (q.tile_rows + MT * 16 - 1) / (MT * 16), most = 224 * 1024 / (kSmem + 1024), held = MT == 1 ? 4 : 3;
+  const int64_t slots = (int64_t)(most < held ? most : held) * processors();
+  auto chunks_of = [&](int per_warp) {
+    int chunks = 0;
+    for (int p = 0; p < q.parts.n; ++p) {
+      const int here = (q.parts.end[p] - (p ? q.parts.end[p - 1] : 0) + 31) / 32;
+      chunks += (here + per_warp * kUpWarps - 1) / (per_warp * kUpWarps);
+    }
+    return chunks;
+  };
+  int per_warp = 1;
+  int64_t least = 0;
+  for (int n = 1; n <= 16; ++n) {
+    const int64_t blocks = (int64_t)q.n_tiles * subs * chunks_of(n), cost = (blocks + slots - 1) / slots * (n + 2);
+    if (n == 1 || cost < least) per_warp = n, least = cost;
   }
+  const int chunks = chunks_of(per_warp);
   launch_kernel(kernel, dim3(q.n_tiles * subs * chunks), dim3(kUpThreads), kSmem, q.stream, (TY*)q.y, q.ldy, q.h, q.b, q.ranks, q.rows, q.tiles, q.tokens, q.listed, q.slots,
-                q.parts, q.tile_rows, subs, (int)per_warp, chunks, q.rank);
+                q.parts, q.tile_rows, subs, per_warp, chunks, q.rank);
 }
 template <typename TY, int SPLIT>
-static int launch_adapters(const AdapterCall& q, int units) {
+static int launch_adapters(const AdapterCall& q) {
   const bool few = q.tile_rows <= 16;
   const int wide = q.parts.n * ((q.rank + 7) & ~7);
   static_assert(kAdapterMaxWidth == 512, "the last forms cover all of h");
@@ -664,11 +677,11 @@ static int launch_adapters(const AdapterCall& q, int units) {
   int rc = check_launch("adapters_add");
   if (rc != ROOST_OK) return rc;
   if (q.rank <= 32) {
-    few ? launch_adapters_up<TY, SPLIT, 1, 1>(q, units) : launch_adapters_up<TY, SPLIT, 4, 1>(q, units);
+    few ? launch_adapters_up<TY, SPLIT, 1, 1>(q) : launch_adapters_up<TY, SPLIT, 4, 1>(q);
   } else if (q.rank <= 64) {
-    few ? launch_adapters_up<TY, SPLIT, 1, 2>(q, units) : launch_adapters_up<TY, SPLIT, 2, 2>(q, units);
+    few ? launch_adapters_up<TY, SPLIT, 1, 2>(q) : launch_adapters_up<TY, SPLIT, 2, 2>(q);
   } else {
-    few ? launch_adapters_up<TY, SPLIT, 1, 0>(q, units) : launch_adapters_up<TY, SPLIT, 4, 0>(q, units);
+    few ? launch_adapters_up<TY, SPLIT, 1, 0>(q) : launch_adapters_up<TY, SPLIT, 4, 0>(q);
   }
   return check_launch("adapters_add");
 }
@@ -721,7 +734,7 @@ extern "C" int roost_adapters_add(void* y, int64_t ldy, const void* x, int64_t l
     const AdapterCall q{y,    ldy,     (const __nv_bfloat16*)x, ldx,       (const __nv_bfloat16*)a, (const __nv_bfloat16*)b, (__nv_bfloat16*)h, scales, ranks,
                         rows, tiles, n_tiles,                 tile_rows, listed,                  tokens,                  slots,             rank,   inputs,
                         parts, (cudaStream_t)stream};
-    return y_dtype == ROOST_BF16 ? launch_adapters<__nv_bfloat16, 2>(q, (int)units) : launch_adapters<float, 3>(q, (int)units);
+    return y_dtype == ROOST_BF16 ? launch_adapters<__nv_bfloat16, 2>(q) : launch_adapters<float, 3>(q);
   }
   const size_t smem = (size_t)tile_rows * n_parts * rank * sizeof(float);
   ROOST_DISPATCH_DTYPE(dtype, T, ROOST_DISPATCH_DTYPE(y_dtype, TY, {
