@@ -106,6 +106,7 @@ class StepBatch:
     max_kv_len: int = 0
     kv_cap: int = 0              # the bound on the requests' lengths a captured step of this size is made for
     all_single: bool = False     # every row brings exactly one token
+    adapters: object = None      # ``AdapterPlan``: which tokens have which adapter; None: no token has one
     host_buffer: object = None   # the pinned staging buffer, kept until the step is done
     # key -> (the mixer that made it, what it bound): per-step work lists of mixers whose kernels want them, made by the
     # first run that asks and shared by every run that asks under the same key (see ``Mixer.step_work_arrays``)
@@ -151,6 +152,7 @@ class HostTables:
     row_counts: list
     max_position: int
     max_kv_len: int
+    adapter_rows: int = 0        # tokens a tile of the adapters' lists has at most; 0: no row has an adapter
 
 
 class StaticTables:
@@ -210,9 +212,20 @@ class StaticTables:
 class BatchBuilder:
     """Derives a step's tables and places them: a fresh pinned buffer copied to the device once, or a StaticTables."""
 
-    def __init__(self, device, cache_manager):
+    def __init__(self, device, cache_manager, adapter_of: dict | None = None):
+        """``adapter_of``: request id -> adapter slot, of a model with room for adapters: its tables end in the adapters' lists."""
         self.device = torch.device(device)
         self.cm = cache_manager
+        self.adapter_of = adapter_of
+
+    @staticmethod
+    def adapter_tile_rows(num_tokens: int) -> int:
+        """Tokens of a tile of the adapters' lists, by the step's size alone (a captured step's kernels are chosen by it)."""
+        from ..kernels.library import ADAPTER_FEW_ROWS, ADAPTER_FEW_TILES, ADAPTER_TILE_ROWS
+        return ADAPTER_FEW_ROWS if num_tokens <= ADAPTER_FEW_ROWS * ADAPTER_FEW_TILES else ADAPTER_TILE_ROWS
+
+    def uses_adapters(self, request_ids) -> bool:
+        return bool(self.adapter_of) and any(rid in self.adapter_of for rid in request_ids)
 
     def host_tables(self, rows: list[tuple], vocab: int) -> HostTables:
         """rows: (request cache, start position, token list, wanted offsets within the tokens)."""
@@ -272,9 +285,16 @@ class BatchBuilder:
                 scratch = self.cm.pools[gi].capacity       # the slot beyond the pool's: padding rows' state goes there
                 arrays.append(np.asarray([rc.slots[gi] if rc is not None else scratch for rc, *_ in rows], np.int32))
                 arrays.append(np.asarray([1 if rc is not None and start == 0 else 0 for rc, start, *_ in rows], np.int32))
+        adapter_rows = 0
+        if self.adapter_of is not None:
+            from ..kernels.library import adapter_lists
+            slots = [-1 if rc is None else self.adapter_of.get(rc.request_id, -1) for rc, *_ in rows]
+            listed, tiles, tile_rows = adapter_lists([len(r[2]) for r in rows], slots, self.adapter_tile_rows(T))
+            arrays += [listed, tiles.reshape(-1)]
+            adapter_rows = tile_rows if tiles.size else 0
         return HostTables(arrays=arrays, num_tokens=T, num_rows=B, num_selected=len(selected), row_starts=[r[1] for r in rows],
                           row_counts=[len(r[2]) for r in rows], max_position=max(int(pos.max()), 0) if T else 0,
-                          max_kv_len=int(kv_lens.max()) if B else 0)
+                          max_kv_len=int(kv_lens.max()) if B else 0, adapter_rows=adapter_rows)
 
     def _batch(self, ht: HostTables, views: list, host_buffer) -> StepBatch:
         d_ids, d_pos, d_trow, d_qi, d_kvl, d_sel = views[:6]
@@ -287,7 +307,11 @@ class BatchBuilder:
             else:
                 groups.append(GroupTables(state_slots=rest[0], fresh=rest[1]))
                 rest = rest[2:]
-        return StepBatch(num_tokens=ht.num_tokens, num_rows=ht.num_rows, num_selected=ht.num_selected, ids=d_ids, positions=d_pos,
+        adapters = None
+        if ht.adapter_rows:
+            from ..kernels.library import AdapterPlan
+            adapters = AdapterPlan(rows=rest[0], tiles=rest[1].view(-1, 3), tokens=ht.num_tokens, tile_rows=ht.adapter_rows)
+        return StepBatch(adapters=adapters, num_tokens=ht.num_tokens, num_rows=ht.num_rows, num_selected=ht.num_selected, ids=d_ids, positions=d_pos,
                          token_row=d_trow, q_indptr=d_qi, kv_lens=d_kvl, selected=d_sel, groups=groups, row_starts=ht.row_starts,
                          row_counts=ht.row_counts, max_position=ht.max_position, max_kv_len=ht.max_kv_len,
                          kv_cap=graph_kv_cap(ht.max_kv_len), all_single=all(n == 1 for n in ht.row_counts), host_buffer=host_buffer)
@@ -321,11 +345,18 @@ class BatchBuilder:
                 caps += [T, B + 1, B * (-(-kv_cap // g.page_size))]
             else:
                 caps += [B, B]
+        if self.adapter_of is not None:      # every token listed; a part-filled tile a row beside the full ones
+            caps += [T, 3 * (B + T // self.adapter_tile_rows(T))]
         return caps
+
+    def table_fills(self, num_sections: int) -> list[int]:
+        """What fills the sections of a captured step beyond a step's own entries: an unused tile of the adapters' lists names slot -1."""
+        return [0] * num_sections if self.adapter_of is None else [0] * (num_sections - 2) + [-1, -1]
 
     def static_batch(self, ht: HostTables, static: StaticTables, n_table_sections: int) -> StepBatch:
         """A batch over the fixed tables, with the counts of the step they were made for (``ht`` filled up with padding
         rows): every table at its capacity, as many logits as rows."""
         full = HostTables(arrays=ht.arrays, num_tokens=ht.num_tokens, num_rows=ht.num_rows, num_selected=ht.num_rows,
-                          row_starts=ht.row_starts, row_counts=ht.row_counts, max_position=ht.max_position, max_kv_len=ht.max_kv_len)
+                          row_starts=ht.row_starts, row_counts=ht.row_counts, max_position=ht.max_position, max_kv_len=ht.max_kv_len,
+                          adapter_rows=ht.adapter_rows)
         return self._batch(full, static.views[:n_table_sections], None)

@@ -20,6 +20,7 @@ from typing import Iterator
 import torch
 
 from ..sampling.sampler import Sampler, SamplingRow
+from ..parts.adapters import AdapterError
 from .executor import StepEntry, StepExecutor
 from .model import Model, load_model
 from .request import GREEDY, Request, RequestError, SamplingParameters, TokenEvent
@@ -59,6 +60,7 @@ class GenerationOptions:
     logprobs: bool = False                     # the logprob of every generated token
     top_logprobs: int = 0                      # and of this many most likely alternatives (needs logprobs)
     allowed_token_ids: tuple | None = None     # the only tokens that may be generated; None: all
+    adapter: str | None = None                 # the adapter to run with (``RoostEngine.load_adapter``); None: the model as it is
 
     def sampling(self) -> SamplingParameters:
         return SamplingParameters(temperature=self.temperature or 0.0, top_p=1.0 if self.top_p is None else self.top_p,
@@ -67,7 +69,7 @@ class GenerationOptions:
                                   repetition_penalty=1.0 if self.repetition_penalty is None else self.repetition_penalty,
                                   frequency_penalty=self.frequency_penalty or 0.0, presence_penalty=self.presence_penalty or 0.0,
                                   logprobs=self.logprobs, top_logprobs=self.top_logprobs,
-                                  allowed_token_ids=None if self.allowed_token_ids is None else tuple(self.allowed_token_ids))
+                                  allowed_token_ids=None if self.allowed_token_ids is None else tuple(self.allowed_token_ids), adapter=self.adapter)
 
 
 @dataclass
@@ -94,9 +96,11 @@ class Completion:
 class RoostEngine:
     def __init__(self, model, *, dtype: str | torch.dtype = "bfloat16", device: str = "cuda", page_size: int = 16,
                  attention_blocks: int | None = None, kv_fraction: float = 0.9, max_sequences: int = 64, max_tokens: int = 2048,
-                 max_chunk_tokens: int | None = None, seed: int | None = None, chain_steps: bool = True, weights: str = "stored"):
+                 max_chunk_tokens: int | None = None, seed: int | None = None, chain_steps: bool = True, weights: str = "stored",
+                 adapter_slots: int = 0, adapter_rank: int = 16):
         """``model``: a folder with config.json and model.safetensors, or a built ``Model``. ``weights``: "stored", or "e4m3" for the layers'
-        projections in 8 bits with a scale an output row (``load_model``; a built ``Model`` has its form already). ``attention_blocks``:
+        projections in 8 bits with a scale an output row (``load_model``; a built ``Model`` has its form already). ``adapter_slots``: room for that many low-rank adapters
+        of up to ``adapter_rank`` (``load_adapter``). ``attention_blocks``:
         pages in each paged pool (else ``kv_fraction`` of the free device memory); ``max_tokens`` and
         ``max_sequences``: the largest token and row count of a step (the reference's worker flags of the same
         names, src/Starlings.Roost.WorkerHost/WorkerArguments.cs:51-58). ``chain_steps``: while every live request
@@ -108,7 +112,8 @@ class RoostEngine:
             dtype = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}[dtype]
         if isinstance(model, Model) and weights != "stored" and model.rt.weights != weights:
             raise ValueError(f"the model was built with weights {model.rt.weights!r}, not {weights!r}")
-        self.model: Model = model if isinstance(model, Model) else load_model(model, dtype, device, weights=weights)
+        self.model: Model = model if isinstance(model, Model) else load_model(
+            model, dtype, device, weights=weights, adapters=(adapter_slots, adapter_rank) if adapter_slots else None)
         self.executor = StepExecutor(self.model, page_size=page_size, num_pages=attention_blocks, max_requests=max_sequences,
                                      kv_fraction=kv_fraction)
         spec = self.model.spec
@@ -140,8 +145,16 @@ class RoostEngine:
                 raise RequestError("InvalidOption", f"prompt token id {t} is outside the vocabulary of {vocab}")
         if sampling.allowed_token_ids is not None and any(int(t) >= vocab for t in sampling.allowed_token_ids):
             raise RequestError("InvalidOption", f"an allowed token id is outside the vocabulary of {vocab}")
+        slot = None
+        if sampling.adapter is not None:
+            names = self.model.rt.adapters.names if self.model.rt.adapters is not None else {}
+            if sampling.adapter not in names:
+                raise RequestError("InvalidOption", f"adapter {sampling.adapter!r} is not loaded (loaded: {', '.join(sorted(map(str, names))) or 'none'})")
+            slot = names[sampling.adapter]
         req = Request(request_id, [int(t) for t in prompt_token_ids], sampling, tuple(stop_token_ids), priority, deadline)
         self.scheduler.add(req)
+        if slot is not None:
+            self.executor.adapter_of[request_id] = slot
         # a request without a seed gets an engine-chosen one (src/Starlings.Generation.Roost/RoostChatClient.cs:329)
         self._seeds[request_id] = sampling.seed if sampling.seed is not None else self._seed_source.getrandbits(64)
         return request_id
@@ -151,7 +164,28 @@ class RoostEngine:
         self._release(request_id)
         return self.scheduler.cancel(request_id)
 
+    # ------------------------------------------------------------------ adapters
+    def load_adapter(self, name, folder) -> None:
+        """Loads a low-rank adapter (adapter_config.json and adapter_model.safetensors in ``folder``) under ``name``; requests name it in
+        ``GenerationOptions.adapter``. A step mixes requests of any adapters and of none. A name that is loaded already is replaced, but not while a
+        request uses it."""
+        self._idle_adapter(name)
+        self.model.load_adapter(name, folder)
+
+    def unload_adapter(self, name) -> None:
+        """Frees the adapter's slot."""
+        self._idle_adapter(name)
+        if self.model.rt.adapters is None or self.model.rt.adapters.names.pop(name, None) is None:
+            raise AdapterError(f"adapter {name!r} is not loaded")
+
+    def _idle_adapter(self, name) -> None:
+        slots = self.model.rt.adapters
+        if slots is not None and name in slots.names and slots.names[name] in self.executor.adapter_of.values():
+            raise AdapterError(f"adapter {name!r} is in use")
+
     def _release(self, request_id) -> None:
+        if self.executor.adapter_of is not None:
+            self.executor.adapter_of.pop(request_id, None)
         release = getattr(self.sampler, "release", None)
         if release is not None:
             release(request_id)

@@ -93,7 +93,7 @@ class StepGraph:
         builder = executor.builder
         table_caps = builder.table_caps(num_tokens, num_rows, kv_cap)
         self.n_table = len(table_caps)
-        caps, fills = list(table_caps), [0] * len(table_caps)
+        caps, fills = list(table_caps), builder.table_fills(len(table_caps))
         self.work_sections = []             # per set of lists: the indices of its sections
         for key, mixer in self.work:
             sizes = mixer.step_work_caps(key, num_tokens, num_rows, kv_cap, step_class)
@@ -185,7 +185,9 @@ class StepExecutor:
         capacities = [num_pages if g.kind == "paged" else max_requests for g in self.groups]
         self.cache = CacheManager(self.groups, capacities)
         self.storage = CacheStorage(self.groups, capacities, self.rt.dtype, self.rt.device)
-        self.builder = BatchBuilder(self.rt.device, self.cache)
+        # request id -> adapter slot of the requests that use one; None for a model without room for adapters
+        self.adapter_of: dict | None = {} if getattr(self.rt, "adapters", None) is not None else None
+        self.builder = BatchBuilder(self.rt.device, self.cache, self.adapter_of)
         self.steps_run = 0
         self.last_upload_bytes = 0
         # steps are replayed from captured graphs when every part says that its call can be captured and every mixer
@@ -278,7 +280,7 @@ class StepExecutor:
         ht = self.builder.host_tables(padded_rows(rows, tokens_cap, rows_cap), self.model.spec.vocab)
         # what the mixers say about the step's rows decides which of their kernels a step needs at all (a step without
         # short rows is captured without the kernel that serves them): it is part of the captured step's identity
-        key = (tokens_cap, rows_cap, graph_kv_cap(ht.max_kv_len), self.step_class([len(r[2]) for r in rows]))
+        key = (tokens_cap, rows_cap, graph_kv_cap(ht.max_kv_len), self.step_class([len(r[2]) for r in rows], [r[0].request_id for r in rows]))
         g = self._touch(key)
         if g is None:
             if not decode:
@@ -305,8 +307,8 @@ class StepExecutor:
         self.graph_replays += 1
         return g.run(wanted)
 
-    def step_class(self, row_counts: list) -> tuple:
-        out = ()
+    def step_class(self, row_counts: list, request_ids: list = ()) -> tuple:
+        out = (("adapters", True),) if self.builder.uses_adapters(request_ids) else ()
         for m in self.mixers:
             c = m.step_class(row_counts) if hasattr(m, "step_class") else ()
             if c and c not in out:
@@ -352,7 +354,7 @@ class StepExecutor:
         rows = [(self.cache.extend(rid, start + 1), start, [0], [0]) for rid, start in zip(request_ids, starts)]
         cap = graph_rows(len(rows))
         ht = self.builder.host_tables(padded_rows(rows, cap, cap), self.model.spec.vocab)
-        g = self._touch((cap, cap, graph_kv_cap(ht.max_kv_len), self.step_class([1] * len(rows))))
+        g = self._touch((cap, cap, graph_kv_cap(ht.max_kv_len), self.step_class([1] * len(rows), request_ids)))
         if g is None or not g.fits(ht):
             return None
         return PreparedDecode(list(request_ids), starts, g, g.static.stage(g._pending, g.fills))

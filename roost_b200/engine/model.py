@@ -14,6 +14,7 @@ import torch
 from ..config.reader import ConfigReader
 from ..config.spec import ModelSpec
 from ..parts.base import BLOCKS, EMBEDDINGS, HEADS, NORMS, ParamDecl, Runtime
+from ..parts.adapters import AdapterError, place_adapter, read_adapter
 from ..parts.linear import E4m3Linear, Linear
 from .. import registry
 from ..weights import loader as weight_loader
@@ -108,6 +109,27 @@ class Model:
         else:
             self.head.load(placed["lm_head"])
 
+    # ------------------------------------------------------------------ adapters
+    def adapter_projections(self) -> dict:
+        """Module name in the checkpoint -> (the adapters beside its projection, which part of the outputs it is)."""
+        found = {}
+        for i, block in enumerate(self.blocks):
+            for name, part in block.sub_parts().items():
+                for local, stored in self.spec.weight_names.get(f"blocks.{i}.{name}", {}).items():
+                    pool = getattr(getattr(part, local, None), "adapters", None)
+                    if pool is not None:
+                        for p, tensor in enumerate(stored):
+                            found[tensor.removesuffix(".weight")] = (pool, p)
+        return found
+
+    def load_adapter(self, name, folder) -> int:
+        """Loads the adapter in ``folder`` (adapter_config.json, adapter_model.safetensors) under ``name``, in place of what that name held before;
+        returns its slot."""
+        if self.rt.adapters is None:
+            raise AdapterError("the model was built without room for adapters")
+        modules, scale = read_adapter(folder)
+        return place_adapter(self.rt.adapters, self.adapter_projections(), name, modules, scale)
+
     def parts(self):
         """Every part of the model, for questions asked of all of them."""
         yield self.embedding
@@ -177,16 +199,17 @@ def read_model_config(model_dir):
     return arch, cfg, reader
 
 
-def load_model(model_dir, dtype: torch.dtype, device="cuda", kernels=None, weights: str = "stored") -> Model:
+def load_model(model_dir, dtype: torch.dtype, device="cuda", kernels=None, weights: str = "stored", adapters: tuple | None = None) -> Model:
     """Builds the model config.json names and loads model.safetensors into it. ``weights`` "e4m3": the layers' projections in 8 bits (bfloat16
-    models of pre_norm layers of paged attention and gated feed-forwards; the embedding and the head stay as they are)."""
+    models of pre_norm layers of paged attention and gated feed-forwards; the embedding and the head stay as they are). ``adapters`` (slots, rank): room for that many adapters beside the projections of paged
+    attention and gated feed-forwards (``Model.load_adapter``)."""
     from ..kernels import library
     arch, cfg, _ = read_model_config(model_dir)
     tied = getattr(cfg, "tie_word_embeddings", None)
     if tied is None:
         tied = not weight_loader.checkpoint_has(model_dir, "lm_head.weight")
     spec = arch.to_spec(cfg, tied)
-    runtime = Runtime(dtype, device, kernels if kernels is not None else library.load(), weights)
+    runtime = Runtime(dtype, device, kernels if kernels is not None else library.load(), weights, adapters)
     model = Model(spec, runtime)
     decls = parameter_declarations(spec)
     allow = (("lm_head.weight",) if spec.tie_embeddings else ()) + tuple(spec.ignorable_tensors)

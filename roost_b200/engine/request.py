@@ -37,6 +37,7 @@ class SamplingParameters:
     logprobs: bool = False
     top_logprobs: int = 0
     allowed_token_ids: tuple | None = None    # the only tokens that may be generated (the reference's token mask); None: all
+    adapter: object = None                    # the name of the adapter the request is run with; None: the model as it is
 
     MAX_TOP_LOGPROBS = 20
 

@@ -300,9 +300,9 @@ ADAPTER_FEW_ROWS = 16        # ... where tiles of this many still leave processo
 ADAPTER_FEW_TILES = 37
 
 
-def adapter_lists(row_counts: list, row_slots: list) -> tuple:
+def adapter_lists(row_counts: list, row_slots: list, tile_rows: int | None = None) -> tuple:
     """(rows, tiles, tile_rows) of an ``AdapterPlan`` as int32 numpy arrays, for a step whose i-th request brings ``row_counts[i]`` tokens and uses the
-    adapter in slot ``row_slots[i]`` (negative: none)."""
+    adapter in slot ``row_slots[i]`` (negative: none). ``tile_rows``: the most tokens of a tile; None: chosen by the lists."""
     if len(row_counts) != len(row_slots):
         raise KernelError(f"adapter_plan: {len(row_counts)} requests, {len(row_slots)} adapters")
     counts, slots = np.asarray(row_counts, np.int64), np.asarray(row_slots, np.int64)
@@ -317,11 +317,12 @@ def adapter_lists(row_counts: list, row_slots: list) -> tuple:
     def cut(most):
         return [(s, at, min(at + most, end)) for s, lo, end in zip(used, first, ends) for at in range(lo, end, most)]
 
-    tile_rows = ADAPTER_FEW_ROWS
-    tiles = cut(tile_rows)
-    if len(tiles) > ADAPTER_FEW_TILES and max(end - at for _, at, end in tiles) == tile_rows:
-        tile_rows = ADAPTER_TILE_ROWS
-        tiles = cut(tile_rows)
+    tiles = cut(tile_rows or ADAPTER_FEW_ROWS)
+    if tile_rows is None:
+        tile_rows = ADAPTER_FEW_ROWS
+        if len(tiles) > ADAPTER_FEW_TILES and max(end - at for _, at, end in tiles) == tile_rows:
+            tile_rows = ADAPTER_TILE_ROWS
+            tiles = cut(tile_rows)
     return rows.astype(np.int32), np.asarray(tiles, np.int32).reshape(-1, 3), tile_rows
 
 

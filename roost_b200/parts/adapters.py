@@ -1,0 +1,126 @@
+"""Low-rank adapters beside the layers' projections: y[t] += scale[s] B[s] (A[s] x[t]) for the tokens of requests that use the adapter in slot s.
+
+A model that is built with slots keeps room for that many adapters beside every projection that takes them (``AdapterSlots.projection``). An adapter
+is loaded into a slot while the model runs; a step's tokens are dealt out to their adapters by lists that the batch carries (``StepBatch.adapters``), so a
+step may mix requests of any adapters and of none. Adapters are read as they are published: adapter_config.json (``r``, ``lora_alpha``) beside
+adapter_model.safetensors with ``base_model.model.<module>.lora_A.weight`` [r, in] and ``lora_B.weight`` [out, r].
+"""
+from __future__ import annotations
+
+import json
+import math
+from dataclasses import dataclass
+from pathlib import Path
+
+import torch
+
+MAX_PARTS_RANK = 512     # parts times rank that a projection's adapters may have
+
+
+class AdapterError(ValueError):
+    pass
+
+
+@dataclass
+class ProjectionAdapters:
+    """The adapters beside one projection, whose outputs are the parts ``widths`` one after the other."""
+    slots: "AdapterSlots"
+    a: torch.Tensor          # [slots, parts, rank, in]
+    b: torch.Tensor          # [slots, out, rank]
+    widths: tuple
+
+    def add_(self, y: torch.Tensor, x: torch.Tensor, plan) -> torch.Tensor:
+        return self.slots.kernels.adapters_add_(y, x, self.a, self.b, self.slots.scale, plan, widths=self.widths, ranks=self.slots.ranks)
+
+
+class AdapterSlots:
+    """Room for ``slots`` adapters of up to ``rank`` beside the projections of a model."""
+
+    def __init__(self, slots: int, rank: int, dtype: torch.dtype, device, kernels):
+        if slots <= 0 or rank <= 0:
+            raise ValueError(f"adapters: {slots} slots and rank {rank} must be positive")
+        self.count, self.rank = slots, -(-rank // 8) * 8     # rows of whole 16-byte pieces
+        self.dtype, self.device, self.kernels = dtype, device, kernels
+        self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+        self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
+        self.names: dict = {}        # adapter -> slot
+
+    def projection(self, out_features: int, in_features: int, widths: tuple | None = None) -> ProjectionAdapters:
+        widths = (out_features,) if widths is None else tuple(widths)
+        if sum(widths) != out_features:
+            raise ValueError(f"adapters: parts {widths} are not the {out_features} outputs of the projection")
+        if len(widths) * self.rank > MAX_PARTS_RANK:
+            raise ValueError(f"adapters: rank {self.rank} beside a projection of {len(widths)} parts is beyond {MAX_PARTS_RANK // len(widths)}")
+        zeros = lambda *shape: torch.zeros(shape, dtype=self.dtype, device=self.device)
+        return ProjectionAdapters(self, zeros(self.count, len(widths), self.rank, in_features), zeros(self.count, out_features, self.rank), widths)
+
+    def free_slot(self) -> int:
+        for s in range(self.count):
+            if s not in self.names.values():
+                return s
+        raise AdapterError(f"all {self.count} adapter slots are taken ({', '.join(sorted(map(str, self.names)))})")
+
+
+def read_adapter(folder) -> tuple[dict, float]:
+    """(module -> (A, B), scale) of an adapter's folder."""
+    from ..weights.safetensors_io import SafetensorsFile
+    folder = Path(folder)
+    try:
+        config = json.loads((folder / "adapter_config.json").read_text())
+        rank, alpha = int(config["r"]), float(config.get("lora_alpha", config["r"]))
+    except (OSError, ValueError, KeyError, TypeError) as e:
+        raise AdapterError(f"{folder}: adapter_config.json cannot be read ({e})") from None
+    for key in ("use_dora", "modules_to_save", "rank_pattern", "alpha_pattern"):
+        if config.get(key):
+            raise AdapterError(f"{folder}: adapter_config.json asks for {key}, which is not served")
+    if config.get("bias", "none") != "none":
+        raise AdapterError(f"{folder}: adapters with biases are not served")
+    if rank <= 0:
+        raise AdapterError(f"{folder}: rank {rank} must be positive")
+    file = SafetensorsFile(folder / "adapter_model.safetensors")
+    halves: dict = {}
+    for name in file.entries:
+        stem, _, which = name.removesuffix(".weight").rpartition(".")
+        if which not in ("lora_A", "lora_B"):
+            raise AdapterError(f"{folder}: tensor '{name}' is no adapter's")
+        halves.setdefault(stem.removeprefix("base_model.model."), {})[which] = file.tensor(name)
+    for module, pair in halves.items():
+        if len(pair) != 2:
+            raise AdapterError(f"{folder}: '{module}' has one half of an adapter only")
+        if pair["lora_A"].dim() != 2 or pair["lora_B"].dim() != 2 or pair["lora_A"].shape[0] != rank or pair["lora_B"].shape[1] != rank:
+            raise AdapterError(f"{folder}: the adapter of '{module}' is {tuple(pair['lora_A'].shape)} and {tuple(pair['lora_B'].shape)}; expected rank {rank}")
+    return {m: (p["lora_A"], p["lora_B"]) for m, p in halves.items()}, alpha / (math.sqrt(rank) if config.get("use_rslora") else rank)
+
+
+def place_adapter(slots: AdapterSlots, projections: dict, name, modules: dict, scale: float) -> int:
+    """Loads an adapter into a slot of its own (or the one it has) and returns the slot. ``projections``: module name -> (``ProjectionAdapters``, part).
+    Everything is checked before anything is written."""
+    ranks = {a.shape[0] for a, _ in modules.values()}
+    if not modules or len(ranks) != 1:
+        raise AdapterError(f"adapter {name!r}: its modules have ranks {sorted(ranks)}; expected one")
+    rank = ranks.pop()
+    if rank > slots.rank:
+        raise AdapterError(f"adapter {name!r}: rank {rank} is beyond the {slots.rank} that the model has room for")
+    unknown = sorted(set(modules) - set(projections))
+    if unknown:
+        raise AdapterError(f"adapter {name!r}: no projection takes an adapter for {', '.join(unknown[:4])}" + (" and others" if len(unknown) > 4 else ""))
+    for module, (a, b) in modules.items():
+        pool, part = projections[module]
+        want = ((rank, pool.a.shape[3]), (pool.widths[part], rank))
+        if (tuple(a.shape), tuple(b.shape)) != want:
+            raise AdapterError(f"adapter {name!r}: '{module}' is {tuple(a.shape)} and {tuple(b.shape)}; expected {want[0]} and {want[1]}")
+    slot = slots.names[name] if name in slots.names else slots.free_slot()
+    for module, (pool, part) in projections.items():     # a projection the adapter does not name adds nothing
+        lo = sum(pool.widths[:part])
+        rows = slice(lo, lo + pool.widths[part])
+        if module in modules:
+            a, b = modules[module]
+            pool.a[slot, part, :rank].copy_(a.to(device=slots.device, dtype=slots.dtype))
+            pool.b[slot, rows, :rank].copy_(b.to(device=slots.device, dtype=slots.dtype))
+        else:
+            pool.a[slot, part].zero_()
+            pool.b[slot, rows].zero_()
+    slots.scale[slot] = scale
+    slots.ranks[slot] = rank
+    slots.names[name] = slot
+    return slot

@@ -43,7 +43,7 @@ class PagedAttention(Mixer):
         self.rt = runtime
         self.q_width = s.num_heads * s.head_dim
         self.kv_width = s.num_kv_heads * s.head_dim
-        self.qkv = projection(runtime, self.q_width + 2 * self.kv_width, s.hidden)
+        self.qkv = projection(runtime, self.q_width + 2 * self.kv_width, s.hidden, (self.q_width, self.kv_width, self.kv_width))
         self.out = projection(runtime, s.hidden, self.q_width)
         self.q_only = None   # the q rows of qkv, for runs that read another run's cache
         self.q_norm = self.k_norm = None
@@ -89,7 +89,7 @@ class PagedAttention(Mixer):
         if table is None and rotary_dim:
             table = batch.rotation_table(k, inv_freq)
         if write_cache:
-            qkv = self.qkv(x)
+            qkv = self.qkv(x, plan=batch.adapters)
             q = k.qk_norm_rope_cache(qkv, s.num_heads, s.num_kv_heads, s.head_dim, q_w=qw, k_w=kw, eps=eps,
                                      inv_freq=inv_freq, rotary_dim=rotary_dim, positions=batch.positions, cos_sin=table,
                                      k_pool=cache.k_pool, v_pool=cache.v_pool, slot_mapping=tables.slot_mapping,
@@ -100,7 +100,7 @@ class PagedAttention(Mixer):
             q = k.qk_norm_rope_cache(self.q_only(x), s.num_heads, s.num_kv_heads, s.head_dim, q_w=qw, k_w=kw, eps=eps,
                                      inv_freq=inv_freq, rotary_dim=rotary_dim, positions=batch.positions, write_kv=False, cos_sin=table)
         o = self.attend(q, batch, cache, tables)
-        return self.out(o)
+        return self.out(o, plan=batch.adapters)
 
     def attend(self, q, batch, cache, tables):
         """bfloat16 with a head size the tensor-core kernels serve goes to them; float32 and every other head size

@@ -60,7 +60,7 @@ class Runtime:
     """What every part is built with: the compute dtype of activations (and of the cache), the device, and
     the kernel library handle (None only for declaring parameters on a machine without a GPU)."""
 
-    def __init__(self, dtype: torch.dtype, device, kernels=None, weights: str = "stored"):
+    def __init__(self, dtype: torch.dtype, device, kernels=None, weights: str = "stored", adapters: tuple | None = None):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype {dtype} is not float32 or bfloat16")
         if weights not in WEIGHT_FORMS:
@@ -70,6 +70,11 @@ class Runtime:
         # "e4m3": the layers' projections hold their weights in 8 bits with a scale an output row and take rows in 8 bits
         # (parts that say ``serves_e4m3``)
         self.weights = weights
+        # (slots, rank): room for that many adapters beside the projections that take them
+        self.adapters = None
+        if adapters is not None:
+            from .adapters import AdapterSlots
+            self.adapters = AdapterSlots(*adapters, dtype, torch.device(device), kernels)
         self.dtype = dtype
         self.device = torch.device(device)
         self.kernels = kernels

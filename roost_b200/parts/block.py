@@ -34,13 +34,14 @@ class PreNormBlock(Block):
         """``h`` is the previous branch output (or the embedding), ``residual`` the stream before it was added
         (None at the first block). Returns the feed-forward's output and the stream it is still to be added to."""
         if self.rt.e4m3:      # the norms hand their rows over in 8 bits
+            keep = batch.adapters is not None
             if residual is None:
                 residual = h
-                x = self.input_norm.rows_e4m3(h)
+                x = self.input_norm.rows_e4m3(h, keep)
             else:
-                x, residual = self.input_norm.add_norm_e4m3(h, residual)
+                x, residual = self.input_norm.add_norm_e4m3(h, residual, keep)
             a = self.mixer(x, batch, cache, write_cache)
-            y, residual = self.post_mixer_norm.add_norm_e4m3(a, residual)
+            y, residual = self.post_mixer_norm.add_norm_e4m3(a, residual, keep)
             return self.feed_forward(y, batch), residual
         if residual is None:
             residual = h

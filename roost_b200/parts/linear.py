@@ -26,6 +26,7 @@ class Linear:
         self.in_features = in_features
         self.weight: torch.Tensor | None = None
         self.bias: torch.Tensor | None = None
+        self.adapters = None     # ``ProjectionAdapters``, where the model has room for them (``projection``)
 
     def load(self, weight: torch.Tensor, bias: torch.Tensor | None = None) -> None:
         if tuple(weight.shape) != (self.out_features, self.in_features):
@@ -37,7 +38,13 @@ class Linear:
             self.bias = bias.to(self.rt.dtype).contiguous()
             self.bias32 = bias.float().contiguous()
 
-    def __call__(self, x: torch.Tensor, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, out_dtype: torch.dtype | None = None, plan=None) -> torch.Tensor:
+        """``plan``: which tokens have which adapter in this step (``StepBatch.adapters``); None: none has one."""
+        if plan is not None and self.adapters is not None:
+            return self.adapters.add_(self._with_bias(x, out_dtype), x, plan)
+        return self._with_bias(x, out_dtype)
+
+    def _with_bias(self, x: torch.Tensor, out_dtype: torch.dtype | None) -> torch.Tensor:
         if self.bias is None:
             return self._product(x, out_dtype)
         # the bias joins the 32-bit sums before the one rounding: the library product's epilogue in bfloat16, a kernel over
@@ -83,15 +90,18 @@ class Linear:
 
     def first_rows(self, n: int) -> "Linear":
         """A projection onto the first ``n`` outputs, over the same weight."""
+        if self.adapters is not None:
+            raise ValueError("linear: adapters beside a part of a projection's outputs are not served")
         part = Linear(self.rt, n, self.in_features)
         part.load(self.weight[:n])
         return part
 
 
 class E4m3Rows(NamedTuple):
-    """Rows in 8 bits: row t stands for q[t] * scale[t] (``KernelLibrary.quantise_e4m3``)."""
+    """Rows in 8 bits: row t stands for q[t] * scale[t] (``KernelLibrary.quantise_e4m3``). ``plain``: the rows themselves, where adapters read them."""
     q: torch.Tensor
     scale: torch.Tensor
+    plain: torch.Tensor | None = None
 
 
 class E4m3Linear:
@@ -104,26 +114,36 @@ class E4m3Linear:
         self.in_features = in_features
         self.weight: torch.Tensor | None = None      # e4m3 [out, in]
         self.scale: torch.Tensor | None = None       # float32 [out]
+        self.adapters = None
 
     def load(self, weight: torch.Tensor) -> None:
         if tuple(weight.shape) != (self.out_features, self.in_features):
             raise ValueError(f"linear: weight is {tuple(weight.shape)}; expected {(self.out_features, self.in_features)}")
         self.weight, self.scale = self.rt.kernels.quantise_e4m3(weight.to(self.rt.dtype).contiguous())
 
-    def __call__(self, x, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    def __call__(self, x, out_dtype: torch.dtype | None = None, plan=None) -> torch.Tensor:
         k = self.rt.kernels
-        q, scale = x if isinstance(x, E4m3Rows) else k.quantise_e4m3(x)
-        return k.gemm_e4m3(q, scale, self.weight, self.scale, out_dtype or self.rt.dtype)
+        rows = x if isinstance(x, E4m3Rows) else E4m3Rows(*k.quantise_e4m3(x), x)
+        y = k.gemm_e4m3(rows.q, rows.scale, self.weight, self.scale, out_dtype or self.rt.dtype)
+        if plan is not None and self.adapters is not None:
+            self.adapters.add_(y, rows.plain, plan)
+        return y
 
     def first_rows(self, n: int) -> "E4m3Linear":
+        if self.adapters is not None:
+            raise ValueError("linear: adapters beside a part of a projection's outputs are not served")
         part = E4m3Linear(self.rt, n, self.in_features)
         part.weight, part.scale = self.weight[:n], self.scale[:n]
         return part
 
 
-def projection(runtime: Runtime, out_features: int, in_features: int):
-    """A layer's projection without a bias, in the form ``Runtime.weights`` asks for."""
-    return (E4m3Linear if runtime.e4m3 else Linear)(runtime, out_features, in_features)
+def projection(runtime: Runtime, out_features: int, in_features: int, widths: tuple | None = None):
+    """A layer's projection without a bias, in the form ``Runtime.weights`` asks for, with room for adapters where the model has it (``widths``: the
+    parts of its outputs that have adapters of their own)."""
+    part = (E4m3Linear if runtime.e4m3 else Linear)(runtime, out_features, in_features)
+    if runtime.adapters is not None:
+        part.adapters = runtime.adapters.projection(out_features, in_features, widths)
+    return part
 
 
 def batched_linear_f32(rt: Runtime, a: torch.Tensor, w: torch.Tensor) -> torch.Tensor:

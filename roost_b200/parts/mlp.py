@@ -29,14 +29,14 @@ class GatedMlp(FeedForward):
         self.rt = runtime
         if runtime.e4m3 and spec.activation != "silu":
             raise ValueError(f"gated_mlp: weights in e4m3 serve the activation 'silu', not '{spec.activation}'")
-        self.gate_up = projection(runtime, 2 * spec.intermediate, spec.hidden)
+        self.gate_up = projection(runtime, 2 * spec.intermediate, spec.hidden, (spec.intermediate, spec.intermediate))
         self.down = projection(runtime, spec.hidden, spec.intermediate)
         # In bfloat16 with an intermediate size that is a multiple of 128 the gate and up rows are stored interleaved in
         # blocks of 128, the layout in which the tensor-core product applies SiLU(gate) * up to its accumulator, so that
         # for many rows of x the [T, 2I] product never goes to memory; few rows keep the library product and the
         # SiLU kernel, which reads the same layout.
         k = runtime.kernels
-        self.interleave = 128 if (not runtime.full_precision and not runtime.e4m3 and spec.intermediate % 128 == 0 and spec.hidden % 8 == 0
+        self.interleave = 128 if (not runtime.full_precision and not runtime.e4m3 and runtime.adapters is None and spec.intermediate % 128 == 0 and spec.hidden % 8 == 0
                                   and spec.activation == "silu" and hasattr(k, "gemm_tcgen05_swiglu")) else 0
         self.fused_min_rows = 256   # below this the 128-row tiles are mostly empty and the library product is faster
         # ... and so it is while the product is small: measured on a B200, the library product followed by the SiLU kernel
@@ -71,6 +71,10 @@ class GatedMlp(FeedForward):
 
     def __call__(self, x, batch=None):
         k = self.rt.kernels
+        plan = getattr(batch, "adapters", None)
+        if plan is not None and self.rt.adapters is not None:     # gate and up pass through memory, where their adapters join them
+            y = self.gate_up(x, plan=plan)
+            return self.down(k.silu_mul(y) if self.spec.activation == "silu" else k.gated_act_mul(y, self.spec.activation, float(self.spec.limit)), plan=plan)
         if self.rt.e4m3:
             return self.down(E4m3Rows(*k.silu_mul_e4m3(self.gate_up(x))))
         if self.spec.activation != "silu":

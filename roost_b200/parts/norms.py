@@ -37,13 +37,13 @@ class RmsNorm(Norm):
         out = self.rt.kernels.add_rms_norm(x, residual, self.weight, self.spec.eps, rows)
         return out, residual
 
-    def rows_e4m3(self, x: torch.Tensor) -> E4m3Rows:
-        """The norm's rows in 8 bits, for a projection with weights in 8 bits."""
-        return E4m3Rows(*self.rt.kernels.rms_norm_e4m3(x, self.weight, self.spec.eps))
+    def rows_e4m3(self, x: torch.Tensor, keep: bool = False) -> E4m3Rows:
+        """The norm's rows in 8 bits, for a projection with weights in 8 bits; ``keep``: and as they are, for the adapters beside it."""
+        return E4m3Rows(*self.rt.kernels.rms_norm_e4m3(x, self.weight, self.spec.eps, keep=keep))
 
-    def add_norm_e4m3(self, x: torch.Tensor, residual: torch.Tensor):
+    def add_norm_e4m3(self, x: torch.Tensor, residual: torch.Tensor, keep: bool = False):
         """``add_norm`` with the norm's rows in 8 bits."""
-        return E4m3Rows(*self.rt.kernels.add_rms_norm_e4m3(x, residual, self.weight, self.spec.eps)), residual
+        return E4m3Rows(*self.rt.kernels.add_rms_norm_e4m3(x, residual, self.weight, self.spec.eps, keep=keep)), residual
 
 
 class LayerNorm(Norm):

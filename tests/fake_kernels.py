@@ -54,6 +54,18 @@ class FakeKernels:
     def silu_mul_e4m3(self, x, block=0):
         return self._rows_e4m3(self.silu_mul(x.float(), block))
 
+    def adapters_add_(self, y, x, a, b, scale, plan, widths=None, ranks=None):
+        widths = (y.shape[1],) if widths is None else widths
+        for slot, first, end in plan.tiles.tolist():
+            if slot < 0:
+                continue
+            rank, rows, lo = a.shape[2] if ranks is None else int(ranks[slot]), plan.rows[first:end].long(), 0
+            for p, width in enumerate(widths):
+                h = x[rows].float() @ a[slot, p, :rank].float().T
+                y[rows, lo:lo + width] = (y[rows, lo:lo + width].float() + float(scale[slot]) * (h @ b[slot, lo:lo + width, :rank].float().T)).to(y.dtype)
+                lo += width
+        return y
+
     def gemm_e4m3(self, q, q_scale, w, w_scale, out_dtype=torch.bfloat16):
         return (q.float() @ w.float().T * w_scale * q_scale[:, None]).to(out_dtype)
 
