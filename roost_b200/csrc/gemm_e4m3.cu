@@ -53,11 +53,6 @@ __device__ __forceinline__ uint32_t remote_address(uint32_t addr, uint32_t rank)
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float load_remote(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ void arrive_remote(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
 }
@@ -455,10 +450,10 @@ __global__ void __launch_bounds__(192, 1)
     prefetch_tensormap(&tma_q);
     prefetch_tensormap(&tma_w);
   }
+  pdl_launch_dependents();
+  pdl_wait();      // ahead of the tensor memory: whoever holds it may be waiting for nothing but this kernel's predecessors
   if (warp == 1) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), kCols);
   tcgen05_fence_before();
-  pdl_launch_dependents();
-  pdl_wait();
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = tmem_slot;
@@ -563,13 +558,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     prefetch_tensormap(&tma_q);
     prefetch_tensormap(&tma_w);
   }
+  pdl_launch_dependents();
+  pdl_wait();
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"((uint32_t)__cvta_generic_to_shared(&tmem_slot)), "r"(kCols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
   }
   tcgen05_fence_before();
-  pdl_launch_dependents();
-  pdl_wait();
   __syncthreads();
   sync_cluster();  // both CTAs' barriers exist before anyone arrives on the other's
   tcgen05_fence_after();

@@ -629,7 +629,7 @@ int roost_head_gate_mul(void* x, const void* g, int64_t ld_g, int col, int token
 /* ---- rows_e4m3.cu: rows in 8 bits (e4m3) with a scale a row: scale[t] = max(max |v[t, :]| / 448, 2^-126), q[t, i] nearest to v[t, i] / scale[t].
  * A row that holds an infinity or a NaN has a scale that is not finite and makes the row of a product with it NaN. ---- */
 #define ROOST_E4M3_MAX_COLS 51168   /* the longest row these entry points serve */
-/* v = x; rows ldx elements apart, q contiguous. */
+/* v = x; rows ldx elements apart, q contiguous. The kernel behind begins when the rows are written, so that they may be its weight. */
 int roost_quantise_e4m3(const void* x, int64_t ldx, void* q, float* scale, int rows, int cols, int dtype, roost_stream_t stream);
 /* v = silu(gate) * up in 32 bits, x and block as roost_silu_mul. */
 int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tokens, int inter, int block, int dtype, roost_stream_t stream);

@@ -385,11 +385,11 @@ __global__ void __launch_bounds__(1024) rows_e4m3_walk_kernel(const Source src, 
 
 template <typename T, int KV>
 __global__ void __launch_bounds__(1024) quantise_e4m3_vec_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale, int cols) {
-  pdl_launch_dependents();
   const size_t t = blockIdx.x;
   PlainVec<T, KV> row;
   row.x = x + t * ldx;
   row_e4m3_vec<KV>(row, q + t * cols, scale + t, cols, 0.f);
+  rows_are_written();
 }
 template <typename T, int KV>
 __global__ void __launch_bounds__(1024) silu_mul_e4m3_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, int inter, int block, int shift) {
@@ -418,13 +418,19 @@ __global__ void __launch_bounds__(1024) rms_norm_e4m3_vec_kernel(const T* __rest
   row_e4m3_vec<KV>(row, q + t * hidden, scale + t, hidden, eps);
 }
 
+// A weight's rows may go straight into a product, which reads its weight ahead of its wait: the next kernel begins only when the rows are written.
+__device__ __forceinline__ void rows_are_written() {
+  __threadfence();
+  __syncthreads();
+  pdl_launch_dependents();
+}
 template <typename T>
 __global__ void quantise_e4m3_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale, int cols) {
   extern __shared__ float buf[];
-  pdl_launch_dependents();
   pdl_wait();
   const size_t t = blockIdx.x;
   row_e4m3(PlainRow<T>{x + t * ldx}, q + t * cols, scale + t, cols, 0.f, buf);
+  rows_are_written();
 }
 template <typename T>
 __global__ void silu_mul_e4m3_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, int inter, int block) {

@@ -544,6 +544,8 @@ class KernelLibrary:
         if a.dim() != 4 or b.dim() != 3 or a.shape[1] != len(widths) or a.shape[3] != K or tuple(b.shape) != (a.shape[0], N, a.shape[2]) or sum(widths) != N:
             raise KernelError(f"adapters_add_: a {tuple(a.shape)}, b {tuple(b.shape)} and widths {widths} do not fit x {tuple(x.shape)} and y {tuple(y.shape)}")
         S, P, R, _ = a.shape
+        if y.data_ptr() == x.data_ptr() and y.numel():
+            raise KernelError("adapters_add_: y and x are the same memory")
         if x.shape[0] != T or plan.tokens > T or scale.numel() != S:
             raise KernelError(f"adapters_add_: y has {T} rows, x {x.shape[0]}, the plan {plan.tokens}; {scale.numel()} scales for {S} slots")
         if ranks is not None:

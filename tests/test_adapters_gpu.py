@@ -151,7 +151,7 @@ def test_refusals(kernels):
     plan, ranks = kernels.adapter_plan([2, 2], [0, 1]), torch.zeros(2, dtype=torch.int32, device="cuda")
     ok = dict(y=y, x=x, a=a, b=b, scale=scale, plan=plan)
     wide = rand((2, 1, 520, 64), torch.bfloat16, 3)
-    for change in (dict(x=x[:3]), dict(x=x.float()), dict(a=a[:, :, :, :32].contiguous()), dict(b=b[:1]), dict(b=b.float()), dict(scale=scale.double()), dict(scale=scale[:1]),
+    for change in (dict(y=x, b=rand((2, 64, 8), torch.bfloat16, 4)), dict(x=x[:3]), dict(x=x.float()), dict(a=a[:, :, :, :32].contiguous()), dict(b=b[:1]), dict(b=b.float()), dict(scale=scale.double()), dict(scale=scale[:1]),
                    dict(widths=(64, 32)), dict(widths=(95,)), dict(ranks=ranks[:1]), dict(ranks=ranks.long()), dict(y=y.cpu()), dict(y=y.half()),
                    dict(plan=kernels.adapter_plan([9], [0])), dict(a=wide, b=rand((2, 96, 520), torch.bfloat16, 1))):
         with pytest.raises(KernelError):

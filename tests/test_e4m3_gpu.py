@@ -190,6 +190,23 @@ def test_product_keeps_a_rows_nan_to_itself(kernels):
         assert torch.equal(got[keep], clean[keep])
 
 
+@pytest.mark.parametrize("m", [4, 48, 300])
+def test_a_weight_is_multiplied_right_after_it_is_quantised(kernels, m):
+    """A product reads its weight ahead of the wait for the kernel in front, which here is the one that writes it."""
+    q, q_scale = kernels.quantise_e4m3(rand((m, 4096), torch.float32, 1))
+    stored = [rand((4096, 4096), torch.bfloat16, 10 + i) for i in range(4)]
+    wants = []
+    for w in stored:
+        made = kernels.quantise_e4m3(w)
+        torch.cuda.synchronize()
+        wants.append(kernels.gemm_e4m3(q, q_scale, *made))
+        del made
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for w, want in zip(stored, wants):
+            assert torch.equal(kernels.gemm_e4m3(q, q_scale, *kernels.quantise_e4m3(w)), want)
+
+
 def test_no_rows(kernels):
     x = torch.empty((0, 256), dtype=torch.bfloat16, device="cuda")
     w = torch.ones(256, dtype=torch.bfloat16, device="cuda")
