@@ -62,6 +62,12 @@ __device__ __forceinline__ void block_sum_top(float& sum, float& top_value, floa
   top_value = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nwarps ? scratch_top[lane] : 0u));
 }
 
+// A weight's rows may go straight into a product, which reads its weight ahead of its wait: the next kernel begins only when the rows are written.
+__device__ __forceinline__ void rows_are_written() {
+  __threadfence();
+  __syncthreads();
+  pdl_launch_dependents();
+}
 // What a row is made of. load(i): the number before the row's factor (the norm's 1 / sqrt), `square`: what enters the mean square.
 template <typename T>
 struct PlainRow {
@@ -418,12 +424,6 @@ __global__ void __launch_bounds__(1024) rms_norm_e4m3_vec_kernel(const T* __rest
   row_e4m3_vec<KV>(row, q + t * hidden, scale + t, hidden, eps);
 }
 
-// A weight's rows may go straight into a product, which reads its weight ahead of its wait: the next kernel begins only when the rows are written.
-__device__ __forceinline__ void rows_are_written() {
-  __threadfence();
-  __syncthreads();
-  pdl_launch_dependents();
-}
 template <typename T>
 __global__ void quantise_e4m3_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale, int cols) {
   extern __shared__ float buf[];
