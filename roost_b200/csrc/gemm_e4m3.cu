@@ -79,6 +79,12 @@ __device__ __forceinline__ void let_copies_land(volatile int* abortp) {
 // shared memory (4 KB a warp, 16-byte pieces swizzled by their row), so that eight lanes write a row's 128 bytes together: a store of 16 bytes of
 // 32 rows at once takes 32 turns where this takes 4, and the last tile's stores are not hidden by another tile.
 constexpr uint32_t kStoreBytes = 4 * 32 * 128;
+// The tensor cores cut their sums off, so a chain of them leans towards zero with its length: 1.3e-6 of the outputs' norm at a k of 14,640, 4e-7 in
+// two chains of half of it that are added to nearest. 16-bit outputs do not see it; float32 outputs of a long k have two chains, in both accumulators of a
+// tile, so that the next tile's products wait for this one's stores: with the stores' twice as many bytes 4,096 x 4,096 x 12,288 takes 170 us, 152 with
+// 16-bit outputs and one chain; 1,000 x 4,096 x 14,336 50 and 46.
+template <typename TOut>
+__host__ __device__ constexpr bool two_chains(int k) { return sizeof(TOut) == 4 && k > 8192; }
 template <typename TOut, int N>
 __device__ __forceinline__ void put_piece(uint32_t buf, int row, int piece, const float (&o)[N]) {
   uint32_t u[4];
@@ -96,7 +102,7 @@ __device__ __forceinline__ void put_piece(uint32_t buf, int row, int piece, cons
 }
 template <typename TOut, int BN>
 __device__ __forceinline__ void store_rows(TOut* out, int64_t ldo, uint32_t taddr, int row0, int n0, int M, int N, const float* q_scale, const float* w_scale,
-                                           uint32_t buf) {
+                                           uint32_t buf, bool two) {
   constexpr int kVec = 16 / sizeof(TOut), kCols = 8 * kVec;   // columns of 128 bytes
   const int lane = threadIdx.x & 31;
   // rows that start on 16 bytes, else (and at the end of a row) single numbers, neighbours by neighbouring lanes
@@ -111,6 +117,15 @@ __device__ __forceinline__ void store_rows(TOut* out, int64_t ldo, uint32_t tadd
 #pragma unroll
     for (int i = 0; i < kCols / 32; ++i) tcgen05_ld_32x32b_x32_nowait(taddr + c + 32 * i, reinterpret_cast<uint32_t(&)[32]>(v[32 * i]));
     tcgen05_wait_ld();
+    if constexpr (sizeof(TOut) == 4) {
+      if (two) {
+        uint32_t b[kCols];
+        tcgen05_ld_32x32b_x32_nowait(taddr + BN + c, b);
+        tcgen05_wait_ld();
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(b[i]));
+      }
+    }
     if (whole && col + kCols <= N) {
 #pragma unroll
       for (int p = 0; p < 8; ++p) {
@@ -459,6 +474,7 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t tmem = tmem_slot;
   volatile int* abortp = &abort_flag;
   const int m_tiles = (M + 127) / 128, n_tiles = (N + BN - 1) / BN, kbs = (K + kBlockK - 1) / kBlockK, tiles = m_tiles * n_tiles;
+  const int chains = two_chains<TOut>(K) ? 2 : 1;      // accumulators of a tile
 
   if (warp == 0) {
     if (lane == 0) {
@@ -483,18 +499,19 @@ __global__ void __launch_bounds__(192, 1)
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++it) {
-        const int acc = it & 1;
+      const int units = blockIdx.x < tiles ? ((tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1) * chains : 0;
+      for (; it < units && ok; ++it) {
+        const int acc = it & 1, part = chains == 2 ? acc : 0, kb0 = kbs * part / chains, kb1 = kbs * (part + 1) / chains;
         if (!(ok = mbar_wait_limited(acc_empty(acc), ((uint32_t)(it >> 1) & 1u) ^ 1u, abortp, 2, error))) break;
         tcgen05_fence_after();
-        for (int kb = 0; kb < kbs; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = mbar_wait_limited(full(stage), phase, abortp, 3, error))) break;
           tcgen05_fence_after();
           const uint64_t a_desc = umma_desc_k_major_sw128(smem_base + stage * kStage);
           const uint64_t b_desc = umma_desc_k_major_sw128(smem_base + stage * kStage + kStageA);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_e4m3(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            mma_e4m3(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
           tcgen05_commit(empty(stage));
           if (++stage == kStages) stage = 0, phase ^= 1u;
         }
@@ -504,14 +521,19 @@ __global__ void __launch_bounds__(192, 1)
   } else {
     const int lanes = (warp & 3) * 32;
     int it = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++it) {
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, it += chains) {
       const int acc = it & 1, row = (t % m_tiles) * 128 + lanes, n0 = (t / m_tiles) * BN;
       if (!mbar_wait_limited(acc_full(acc), (uint32_t)(it >> 1) & 1u, abortp, 4, error)) break;
+      if (chains == 2 && !mbar_wait_limited(acc_full(1), (uint32_t)(it >> 1) & 1u, abortp, 4, error)) break;
       tcgen05_fence_after();
-      store_rows<TOut, BN>(out, ldo, tmem + ((uint32_t)lanes << 16) + (uint32_t)(acc * BN), row, n0, M, N, q_scale, w_scale, smem_base + kStages * kStage + lanes * 128);
+      store_rows<TOut, BN>(out, ldo, tmem + ((uint32_t)lanes << 16) + (uint32_t)(acc * BN), row, n0, M, N, q_scale, w_scale, smem_base + kStages * kStage + lanes * 128,
+                             chains == 2);
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty(acc));
+      if (lane == 0) {
+        mbar_arrive(acc_empty(acc));
+        if (chains == 2) mbar_arrive(acc_empty(1));
+      }
     }
   }
   __syncwarp();
@@ -571,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   const uint32_t tmem = tmem_slot;
   volatile int* abortp = &abort_flag;
   const int m_tiles = (M + 255) / 256, n_tiles = (N + 255) / 256, kbs = (K + kBlockK - 1) / kBlockK, tiles = m_tiles * n_tiles;
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, chains = two_chains<TOut>(K) ? 2 : 1;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -597,18 +619,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; t < tiles && ok; t += pairs, ++it) {
-        const int acc = it & 1;
+      const int units = pair < tiles ? ((tiles - 1 - (int)pair) / (int)pairs + 1) * chains : 0;
+      for (; it < units && ok; ++it) {
+        const int acc = it & 1, part = chains == 2 ? acc : 0, kb0 = kbs * part / chains, kb1 = kbs * (part + 1) / chains;
         if (!(ok = mbar_wait_limited<true>(acc_empty(acc), ((uint32_t)(it >> 1) & 1u) ^ 1u, abortp, 2, error))) break;
         tcgen05_fence_after();
-        for (int kb = 0; kb < kbs; ++kb) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = mbar_wait_limited<true>(full(stage), phase, abortp, 3, error))) break;
           tcgen05_fence_after();
           const uint64_t a_desc = umma_desc_k_major_sw128(smem_base + stage * kStage);
           const uint64_t b_desc = umma_desc_k_major_sw128(smem_base + stage * kStage + kStageA);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_e4m3_pair(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            mma_e4m3_pair(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
           commit_pair(empty(stage));
           if (++stage == kStages) stage = 0, phase ^= 1u;
         }
@@ -619,14 +642,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
     const int lanes = (warp & 3) * 32;
     const uint32_t even_acc_empty[2] = {remote_address(acc_empty(0), 0), remote_address(acc_empty(1), 0)};
     int it = 0;
-    for (int t = pair; t < tiles; t += pairs, ++it) {
+    for (int t = pair; t < tiles; t += pairs, it += chains) {
       const int acc = it & 1, row = (t % m_tiles) * 256 + (int)rank * 128 + lanes, n0 = (t / m_tiles) * 256;
       if (!mbar_wait_limited(acc_full(acc), (uint32_t)(it >> 1) & 1u, abortp, 4, error)) break;
+      if (chains == 2 && !mbar_wait_limited(acc_full(1), (uint32_t)(it >> 1) & 1u, abortp, 4, error)) break;
       tcgen05_fence_after();
-      store_rows<TOut, 256>(out, ldo, tmem + ((uint32_t)lanes << 16) + (uint32_t)(acc * BN), row, n0, M, N, q_scale, w_scale, smem_base + kStages * kStage + lanes * 128);
+      store_rows<TOut, 256>(out, ldo, tmem + ((uint32_t)lanes << 16) + (uint32_t)(acc * BN), row, n0, M, N, q_scale, w_scale, smem_base + kStages * kStage + lanes * 128,
+                             chains == 2);
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_remote(even_acc_empty[acc]);
+      if (lane == 0) {
+        arrive_remote(even_acc_empty[acc]);
+        if (chains == 2) arrive_remote(even_acc_empty[1]);
+      }
     }
   }
   __syncwarp();
@@ -715,11 +743,12 @@ struct Operands {
 // The few-row form: `split` CTAs a tile, as many (up to 8) as leave a processor one CTA, and two blocks of k for each: a processor's second CTA waits for
 // the same tensor cores, and the sums of a cluster cost more than it brings (8 x 4,096 x 4,096: split 4 6.6 us, 8 8.2, 2 8.3; 8 x 12,288 x 4,096:
 // 1 12.7, 2 14.1; 8 x 24,576 x 4,096: 1 19.6, 2 22.9).
-int split_of(int64_t tiles, int k) {
+// At least `least`, where the sums ask for it.
+int split_of(int64_t tiles, int k, int least = 1) {
   const int kbs = (k + kBlockK - 1) / kBlockK;
   int split = 8;
   // clusters of eight and four leave some processors of every group alone: 15 and 33 of them fit 148 at a CTA each
-  while (split > 1 && (tiles * split * 100 > processors() * (int64_t)(split == 8 ? 80 : (split == 4 ? 88 : 100)) || split > kbs / 2)) split /= 2;
+  while (split > least && (tiles * split * 100 > processors() * (int64_t)(split == 8 ? 80 : (split == 4 ? 88 : 100)) || split > kbs / 2)) split /= 2;
   return split;
 }
 
@@ -727,7 +756,7 @@ template <typename TOut, int NTOK>
 int launch_split(const Operands& o) {
   static std::atomic<uint64_t> done{0};
   using Cfg = SplitCfg<NTOK>;
-  const int tiles = (o.n + 127) / 128, chunks = (o.m + NTOK - 1) / NTOK, split = split_of((int64_t)tiles * chunks, o.k);
+  const int tiles = (o.n + 127) / 128, chunks = (o.m + NTOK - 1) / NTOK, split = split_of((int64_t)tiles * chunks, o.k, two_chains<TOut>(o.k) ? 2 : 1);
   const int kbs = (o.k + kBlockK - 1) / kBlockK;
   // Six stages, four for a short part of k (8 x 4,096 x 4,096: 6.6 us, 7.2 with six); where a processor has two CTAs, as many as let both in.
   const size_t sums = split > 1 ? Cfg::kSums : 0, room = ((int64_t)tiles * chunks * split > processors() ? 112 : 224) * 1024 - 1024 - sums;

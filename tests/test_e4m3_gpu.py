@@ -134,9 +134,10 @@ def test_silu_mul(kernels, dtype, tokens, inter, block):
     gate_at = at // block * 2 * block + at % block if block else at
     gate, up = x.double()[:, gate_at], x.double()[:, gate_at + (block or inter)]
     q, scale = kernels.silu_mul_e4m3(x, block)
-    # expf is within 2 units of its last place (four half steps), the sum, the quotient and the product round once each; a gate far below
-    # zero gives a denormal or zero where the formula gives less than the least number, which the 8 bits do not see
-    check_rows(q, scale, gate * torch.sigmoid(gate) * up, 8 * HALF, "silu_mul")
+    # In half steps (2^-24): expf is within 2 units of its last place, 4, and counts by exp(-g) / (1 + exp(-g)) < 1; the sum rounds, 1; its approximate
+    # reciprocal is within a unit, 2; two products round, 2: 9 together. A gate far below zero gives a denormal or zero where the formula gives less
+    # than the least number, which the 8 bits do not see.
+    check_rows(q, scale, gate * torch.sigmoid(gate) * up, 9 * HALF, "silu_mul")
 
 
 SIZES = [(1, 1, 1), (1, 70, 50), (3, 64, 16), (5, 130, 32), (1, 4096, 4096), (8, 129, 208), (16, 1000, 1024), (17, 24, 4112), (31, 6144, 2048), (33, 257, 144),
@@ -165,6 +166,20 @@ def test_product(kernels, out, m, n, k):
     product_check(got, q, q_scale, w, w_scale, f"product {m} x {n} x {k}")
     again = kernels.gemm_e4m3(q, q_scale, w, w_scale, out)
     assert torch.equal(got, again), "the same bits on every run"
+
+
+@pytest.mark.parametrize("m,n,k", [(2, 5000, 12288), (7, 300, 8208), (30, 4100, 9008), (64, 20000, 8320), (90, 264, 16384), (300, 2050, 8208), (520, 4096, 8448),
+                                   (1000, 4096, 14336), (2500, 4100, 8208), (4000, 72, 10240)])
+def test_product_of_a_long_k(kernels, m, n, k):
+    """Tiles, pairs and strips that a processor meets more than once, with two sums a tile; the errors together are below 2^-20 of the outputs."""
+    q, q_scale = kernels.quantise_e4m3(rand((m, k), torch.float32, 8))
+    w, w_scale = kernels.quantise_e4m3(rand((n, k), torch.float32, 9, 0.02))
+    got = kernels.gemm_e4m3(q, q_scale, w, w_scale, torch.float32)
+    product_check(got, q, q_scale, w, w_scale, f"product {m} x {n} x {k}")
+    want = (q.double() @ w.double().t()) * q_scale.double()[:, None] * w_scale.double()
+    assert (got.double() - want).norm() <= 2.0 ** -20 * want.norm()
+    assert torch.equal(got, kernels.gemm_e4m3(q, q_scale, w, w_scale, torch.float32))
+    product_check(kernels.gemm_e4m3(q, q_scale, w, w_scale, torch.bfloat16), q, q_scale, w, w_scale, f"product {m} x {n} x {k}, bfloat16")
 
 
 @pytest.mark.parametrize("m,n,k,pad", [(9, 200, 256, 16), (9, 200, 256, 3), (200, 384, 512, 48), (40, 256, 96, 1)])
@@ -205,6 +220,36 @@ def test_a_weight_is_multiplied_right_after_it_is_quantised(kernels, m):
     for _ in range(5):
         for w, want in zip(stored, wants):
             assert torch.equal(kernels.gemm_e4m3(q, q_scale, *kernels.quantise_e4m3(w)), want)
+
+
+def test_more_rows_than_a_grid_has_in_its_second_direction(kernels):
+    """70,000 rows of the row kernels and of the products' forms, the last rows as well as the first."""
+    x = rand((70000, 64), torch.bfloat16, 1)
+    q, scale = kernels.quantise_e4m3(x)
+    check_rows(q, scale, x.double(), 0.0, "quantise")
+    w = torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    for name, got in (("norm", kernels.rms_norm_e4m3(x, w, 1e-6)), ("silu_mul", kernels.silu_mul_e4m3(x))):
+        few = kernels.rms_norm_e4m3(x[-70:], w, 1e-6) if name == "norm" else kernels.silu_mul_e4m3(x[-70:])
+        assert torch.equal(got[0][-70:].view(torch.uint8), few[0].view(torch.uint8)) and torch.equal(got[1][-70:], few[1]), name
+    wq, ws = kernels.quantise_e4m3(rand((40, 64), torch.float32, 2))
+    product_check(kernels.gemm_e4m3(q, scale, wq, ws), q, scale, wq, ws, "70,000 rows")
+    odd, odd_scale = kernels.quantise_e4m3(x[:, :50].contiguous())
+    wq, ws = kernels.quantise_e4m3(rand((4, 50), torch.float32, 2))
+    product_check(kernels.gemm_e4m3(odd, odd_scale, wq, ws), odd, odd_scale, wq, ws, "70,000 rows of any size")
+    product_check(kernels.gemm_e4m3(wq, ws, odd, odd_scale), wq, ws, odd, odd_scale, "70,000 columns of any size")
+
+
+def test_rows_of_more_than_two_dimensions(kernels):
+    """The norms take them, as the norms of 16-bit outputs do; the others refuse them."""
+    from roost_b200.kernels.library import KernelError
+    x, w = rand((2, 3, 96), torch.bfloat16, 1), rand((96,), torch.bfloat16, 2)
+    for call in (lambda v: kernels.rms_norm_e4m3(v, w, 1e-6), lambda v: kernels.add_rms_norm_e4m3(v, torch.ones_like(v), w, 1e-6)):
+        (q, scale), (flat, flat_scale) = call(x), call(x.reshape(6, 96))
+        assert q.shape[:-1] == scale.shape == (2, 3)
+        assert torch.equal(q.reshape(6, -1).view(torch.uint8), flat.view(torch.uint8)) and torch.equal(scale.reshape(6), flat_scale)
+    for call in (kernels.quantise_e4m3, kernels.silu_mul_e4m3):
+        with pytest.raises(KernelError):
+            call(x)
 
 
 def test_no_rows(kernels):
