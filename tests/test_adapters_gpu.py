@@ -97,6 +97,31 @@ def test_larger_sizes(kernels, dtype, out):
     case(kernels, dtype, out, [300, 211, 2], [3, 0, 2], 4, 32, 2048, (2048, 2048))
 
 
+@pytest.mark.parametrize("dtype,out", TYPES)
+@pytest.mark.parametrize("R,K,widths", [(64, 4096, (2048, 512, 512)), (128, 4104, (1000, 264, 8, 256)), (512, 2056, (640,)), (72, 8200, (96, 5000)), (24, 8, (256,)),
+                                        (64, 1024, (8,) * 8)])
+def test_large_ranks(kernels, dtype, out, R, K, widths):
+    """h is up to 512 numbers a token: few tokens and tiles of 64, ranks that end inside a block of 32, one block of the inputs and many."""
+    ranks = [R, R - 7, 1, 40 if R > 40 else 9]
+    case(kernels, dtype, out, [1, 3, 1, 2, 1], [0, 1, 2, -1, 3], 4, R, K, widths)
+    case(kernels, dtype, out, [1, 3, 1, 2, 1], [0, 1, 2, -1, 3], 4, R, K, widths, ranks=ranks)
+    case(kernels, dtype, out, [70, 1, 64, 90], [1, 2, 3, 0], 4, R, K, widths, ranks=ranks)
+
+
+def test_offsets_beyond_32_bits(kernels):
+    """Rows of y and of b that lie more than 2 ** 31 numbers behind the first."""
+    T, N, R, K, S = 40000, 60000, 8, 64, 5000
+    y = torch.zeros((T, N), dtype=torch.bfloat16, device="cuda")
+    x = rand((T, K), torch.bfloat16, 1)
+    a = rand((S, 1, R, K), torch.bfloat16, 2)
+    b = torch.zeros((S, N, R), dtype=torch.bfloat16, device="cuda")
+    b[-1] = rand((N, R), torch.bfloat16, 3)
+    scale = torch.full((S,), 0.5, device="cuda")
+    kernels.adapters_add_(y, x, a, b, scale, kernels.adapter_plan([T - 5, 5], [-1, S - 1]))
+    want, bound = want_and_bound(torch.zeros_like(y[-5:]), x[-5:], a[-1:], b[-1:], scale[:1], [5], [0], (N,), None, 2.0 ** -17)
+    assert bool(((y[-5:].double() - want).abs() <= bound).all()) and not bool(y[:-5].any())
+
+
 def test_a_list_that_is_wrong_reaches_nothing(kernels):
     """Slots that do not exist and tokens outside the step are passed over."""
     from roost_b200.kernels.library import AdapterPlan

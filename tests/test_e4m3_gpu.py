@@ -239,6 +239,22 @@ def test_more_rows_than_a_grid_has_in_its_second_direction(kernels):
     product_check(kernels.gemm_e4m3(wq, ws, odd, odd_scale), wq, ws, odd, odd_scale, "70,000 columns of any size")
 
 
+@pytest.mark.parametrize("m", [5, 12, 200])
+@pytest.mark.parametrize("k", [32784, 32785])
+def test_a_weight_beyond_32_bits(kernels, m, k):
+    """Rows of a weight that lie more than 2 ** 31 numbers behind its first, and of the rows that it is made from."""
+    n = 66000
+    w = torch.randint(0, 0x40, (n, k), dtype=torch.uint8, device="cuda").view(E4M3)
+    w_scale = torch.ones(n, device="cuda")
+    q, q_scale = kernels.quantise_e4m3(rand((m, k), torch.float32, 1))
+    product_check(kernels.gemm_e4m3(q, q_scale, w, w_scale)[:, -300:], q, q_scale, w[-300:], w_scale[-300:], f"product {m} x {n} x {k}")
+    if m == 5:
+        x = w.to(torch.bfloat16)
+        got, scale = kernels.quantise_e4m3(x)
+        few = kernels.quantise_e4m3(x[-9:].clone())
+        assert torch.equal(got[-9:].view(torch.uint8), few[0].view(torch.uint8)) and torch.equal(scale[-9:], few[1])
+
+
 def test_rows_of_more_than_two_dimensions(kernels):
     """The norms take them, as the norms of 16-bit outputs do; the others refuse them."""
     from roost_b200.kernels.library import KernelError
