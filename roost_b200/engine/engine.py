@@ -99,8 +99,8 @@ class RoostEngine:
                  max_chunk_tokens: int | None = None, seed: int | None = None, chain_steps: bool = True, weights: str = "stored",
                  adapter_slots: int = 0, adapter_rank: int = 16):
         """``model``: a folder with config.json and model.safetensors, or a built ``Model``. ``weights``: "stored", or "e4m3" for the layers'
-        projections in 8 bits with a scale an output row (``load_model``; a built ``Model`` has its form already). ``adapter_slots``: room for that many low-rank adapters
-        of up to ``adapter_rank`` (``load_adapter``). ``attention_blocks``:
+        projections in 8 bits with a scale an output row (``load_model``; a built ``Model`` has its form already). ``adapter_slots``:
+        room for that many low-rank adapters of up to ``adapter_rank`` (``load_adapter``; a built ``Model`` has its room already). ``attention_blocks``:
         pages in each paged pool (else ``kv_fraction`` of the free device memory); ``max_tokens`` and
         ``max_sequences``: the largest token and row count of a step (the reference's worker flags of the same
         names, src/Starlings.Roost.WorkerHost/WorkerArguments.cs:51-58). ``chain_steps``: while every live request
@@ -112,6 +112,8 @@ class RoostEngine:
             dtype = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16, "float32": torch.float32, "fp32": torch.float32}[dtype]
         if isinstance(model, Model) and weights != "stored" and model.rt.weights != weights:
             raise ValueError(f"the model was built with weights {model.rt.weights!r}, not {weights!r}")
+        if isinstance(model, Model) and adapter_slots and (model.rt.adapters is None or model.rt.adapters.count < adapter_slots):
+            raise ValueError(f"the model was built with room for {model.rt.adapters.count if model.rt.adapters is not None else 0} adapters, not {adapter_slots}")
         self.model: Model = model if isinstance(model, Model) else load_model(
             model, dtype, device, weights=weights, adapters=(adapter_slots, adapter_rank) if adapter_slots else None)
         self.executor = StepExecutor(self.model, page_size=page_size, num_pages=attention_blocks, max_requests=max_sequences,

@@ -58,6 +58,8 @@ class Model:
                 if need != owner:
                     raise ValueError(f"schedule entry {n} reads the cache of entry {e.reads_cache_of}, whose geometry differs "
                                      f"({owner} against {need})")
+                if runtime.adapters is not None and getattr(getattr(self.blocks[e.block].mixer, "qkv", None), "adapters", None) is not None:
+                    raise ValueError(f"schedule entry {n} reads the cache of entry {e.reads_cache_of}: adapters beside a part of a projection's outputs are not served")
                 need = None
             self.cache_needs.append(need)
 

@@ -1,14 +1,17 @@
 """Adapters through the engine: requests of several adapters and of none in the same steps, against models whose weights hold the adapter's product."""
+import dataclasses
 import json
 
 import pytest
 import torch
 
 from roost_b200 import GenerationOptions, RoostEngine
+from roost_b200.config.spec import RunEntry
 from roost_b200.engine.executor import StepEntry, StepExecutor
-from roost_b200.engine.model import load_model
+from roost_b200.engine.model import Model, load_model
 from roost_b200.engine.request import RequestError
 from roost_b200.parts.adapters import AdapterError, AdapterSlots
+from roost_b200.parts.base import Runtime
 from roost_b200.weights.safetensors_io import SafetensorsFile, write_safetensors
 from tests.fake_kernels import FakeKernels
 from tests.helpers import BF16_RMS_BOUND, FP32_BOUND, random_ids, rms_error, run_whole, scaled_error
@@ -130,6 +133,12 @@ def test_refusals(tiny_model_dirs, adapters, tmp_path):
     with pytest.raises(ValueError, match="beyond"):
         build(base, torch.float32, "cpu", FakeKernels(), (2, 200))
 
+    spec = small.spec
+    shared = dataclasses.replace(spec, schedule=[RunEntry(block=0), RunEntry(block=1, reads_cache_of=0)])
+    Model(shared, Runtime(torch.float32, "cpu", FakeKernels()))
+    with pytest.raises(ValueError, match="not served"):
+        Model(shared, Runtime(torch.float32, "cpu", FakeKernels(), adapters=(2, 8)))
+
     def changed(name, config=None, rename=None, drop=None):
         f = tmp_path / name
         f.mkdir()
@@ -151,6 +160,8 @@ def test_refusals(tiny_model_dirs, adapters, tmp_path):
 
 def test_engine_requests_name_their_adapter(tiny_model_dirs, adapters):
     model = build(tiny_model_dirs["A"], torch.float32, "cpu", FakeKernels())
+    with pytest.raises(ValueError, match="built with room"):
+        RoostEngine(model, device="cpu", attention_blocks=64, adapter_slots=100)
     engine = RoostEngine(model, device="cpu", attention_blocks=64)
     (one, _), _ = adapters["A"]
     with pytest.raises(RequestError, match="not loaded"):
