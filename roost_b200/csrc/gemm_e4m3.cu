@@ -190,10 +190,10 @@ __device__ __forceinline__ void store_transposed(TOut* dst, int64_t ldo, const u
 
 // ------------------------------------------------------------------------------------------------ a handful of rows
 // Latency is all there is to a product of up to 8 rows of q with a small w: a block takes 16 rows of w, its eight warps the blocks of 64 of k in turn,
-// straight from memory into the registers of mma.sync (m16n8k32): no barrier or copy engine lies between the loads and the products, and the first
-// kRowsDeep blocks of w are on their way before the wait for the kernel that makes q. A lane takes 16 numbers of a row at once; which k a
+// straight from memory into the registers of mma.sync (m16n8k32): no barrier or copy engine lies between the loads and the products, and all of a
+// warp's blocks of w, kRowsDeep at most, are on their way before the wait for the kernel that makes q. A lane takes 16 numbers of a row at once; which k a
 // register of the instruction calls its own does not matter as long as both operands agree. The warps' sums meet in shared memory.
-constexpr int kRowsDeep = 8;
+constexpr int kRowsDeep = 8, kRowsMaxK = 64 * 8 * kRowsDeep;
 __device__ __forceinline__ void mma_e4m3_k32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -210,33 +210,27 @@ __global__ void __launch_bounds__(256, 2)
                           TOut* __restrict__ out, int M, int N, int K, int64_t ldq, int64_t ldw, int64_t ldo) {
   __shared__ float part[8][8][17];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int n0 = blockIdx.x * 16, blocks = (K + 63) / 64;
+  const int n0 = blockIdx.x * 16;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const uint8_t* w0 = w + (int64_t)min(n0 + g, N - 1) * ldw + 16 * c;
   const uint8_t* w1 = w + (int64_t)min(n0 + g + 8, N - 1) * ldw + 16 * c;
   float acc[4] = {};
   uint4 a[kRowsDeep][2];
-  auto fetch = [&](int b0) {
-#pragma unroll
-    for (int i = 0; i < kRowsDeep; ++i) {
-      const int k = (b0 + 8 * i) * 64;
-      const bool in = k + 16 * c < K;
-      a[i][0] = in ? load_stream(w0 + k) : zero;
-      a[i][1] = in ? load_stream(w1 + k) : zero;
-    }
-  };
   pdl_launch_dependents();
-  fetch(warp);
-  pdl_wait();
-  for (int b0 = warp; b0 < blocks; b0 += 8 * kRowsDeep) {
-    if (b0 != warp) fetch(b0);
 #pragma unroll
-    for (int i = 0; i < kRowsDeep; ++i) {
-      const int k = (b0 + 8 * i) * 64 + 16 * c;
-      const uint4 b = g < M && k < K ? *reinterpret_cast<const uint4*>(q + (int64_t)g * ldq + k) : zero;
-      mma_e4m3_k32(acc, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
-      mma_e4m3_k32(acc, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
-    }
+  for (int i = 0; i < kRowsDeep; ++i) {
+    const int k = (warp + 8 * i) * 64;
+    const bool in = k + 16 * c < K;
+    a[i][0] = in ? load_stream(w0 + k) : zero;
+    a[i][1] = in ? load_stream(w1 + k) : zero;
+  }
+  pdl_wait();
+#pragma unroll
+  for (int i = 0; i < kRowsDeep; ++i) {
+    const int k = (warp + 8 * i) * 64 + 16 * c;
+    const uint4 b = g < M && k < K ? *reinterpret_cast<const uint4*>(q + (int64_t)g * ldq + k) : zero;
+    mma_e4m3_k32(acc, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
+    mma_e4m3_k32(acc, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
   }
   part[warp][2 * c][g] = acc[0];
   part[warp][2 * c + 1][g] = acc[1];
@@ -255,34 +249,60 @@ __global__ void __launch_bounds__(256, 2)
 // ------------------------------------------------------------------------------------------------ few rows
 // The weight's bytes are the time, so all that it takes is on its way at once: a cluster of `split` CTAs takes 128 rows of w, CTA r the r-th part of k,
 // two or three CTAs a processor, and every CTA asks for all its stages of w before it waits for the kernel that makes q. CTA o adds up the o-th part
-// of the tile's rows: the others send their sums for it straight from tensor memory into its shared memory and arrive on a barrier there, so that
-// nothing is asked for across the cluster and waited for; it adds them in CTA order.
+// of the tile's rows: every CTA lays its sums into the stages, free by then, and a bulk copy a warp sends the rows of CTA o there, which counts the bytes
+// and adds the parts in CTA order.
 constexpr int kSplitStages = 8;
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;\n" ::: "memory"); }
-__device__ __forceinline__ void send_vec(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+// A piece of this CTA's shared memory to another CTA's, which counts the bytes on its barrier.
+__device__ __forceinline__ void send_bytes(uint32_t to, uint32_t from, uint32_t bytes, uint32_t to_bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(to), "r"(from), "r"(bytes), "r"(to_bar)
+               : "memory");
 }
+// Sums lie [block of up to 32 tokens][row][token], a row's 16-byte pieces swizzled so that the same piece of eight neighbouring rows lies in all banks.
+template <int BLOCK>
+__device__ __forceinline__ int sum_at(int row, int piece) { return row * BLOCK + ((piece ^ (BLOCK == 16 ? (row >> 1) & 3 : row & 7)) << 2); }
 template <int NTOK>
 struct SplitCfg {
   static constexpr uint32_t kStageW = 128 * kBlockK, kStage = kStageW + NTOK * kBlockK;
-  static constexpr int kPitch = NTOK + 4;                        // floats of a row of sums
-  static constexpr uint32_t kSums = 128 * kPitch * 4;            // the sums of all CTAs for this CTA's share: 128 rows in all
+  static constexpr int kBlock = NTOK < 32 ? NTOK : 32;           // tokens sent at a time
+  static constexpr uint32_t kSums = 128 * NTOK * 4;              // the sums of all CTAs for this CTA's share: 128 rows in all
 };
+// The S CTAs' sums of a tile's 128 / S rows from `first` on, [CTA][block][row][token], added in CTA order: a thread of 128 one row (f: its scale), four tokens
+// at a time.
+template <typename TOut, int S, int NTOK>
+__device__ __forceinline__ void add_share(TOut* out, int64_t ldo, const float* sums, const float* q_scales, float f, int M) {
+  constexpr int kShare = 128 / S, kBlock = SplitCfg<NTOK>::kBlock;
+  const int etid = threadIdx.x - 64, row = etid % kShare;
+#pragma unroll 4
+  for (int m = etid / kShare * 4; m < M; m += 4 * S) {
+    float4 part[S];
+#pragma unroll
+    for (int c = 0; c < S; ++c) part[c] = *reinterpret_cast<const float4*>(sums + c * kShare * NTOK + m / kBlock * kShare * kBlock + sum_at<kBlock>(row, m % kBlock / 4));
+    const float4 qs = *reinterpret_cast<const float4*>(q_scales + m);
+#pragma unroll
+    for (int c = 1; c < S; ++c) part[0].x += part[c].x, part[0].y += part[c].y, part[0].z += part[c].z, part[0].w += part[c].w;
+    const float o[4] = {part[0].x * f * qs.x, part[0].y * f * qs.y, part[0].z * f * qs.z, part[0].w * f * qs.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (m + j < M) out[(int64_t)(m + j) * ldo] = from_float<TOut>(o[j]);
+    }
+  }
+}
 template <typename TOut, int NTOK>
 __global__ void __launch_bounds__(192, 2)
     gemm_e4m3_split_kernel(const __grid_constant__ CUtensorMap tma_w, const __grid_constant__ CUtensorMap tma_q, const float* __restrict__ q_scale,
                            const float* __restrict__ w_scale, TOut* __restrict__ out, int M, int N, int K, int64_t ldo, int split, int stages, int* error) {
   using Cfg = SplitCfg<NTOK>;
   constexpr uint32_t kStageW = Cfg::kStageW, kStage = Cfg::kStage, kCols = NTOK < 32 ? 32 : NTOK;
-  constexpr int kPitch = Cfg::kPitch;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t smem_base = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
   const uint32_t sums_base = smem_base + stages * kStage;
-  const float* sums = reinterpret_cast<const float*>(smem_raw + (sums_base - (uint32_t)__cvta_generic_to_shared(smem_raw)));   // [CTA][row of its share][kPitch]
+  const float* sums = reinterpret_cast<const float*>(smem_raw + (sums_base - (uint32_t)__cvta_generic_to_shared(smem_raw)));   // [CTA][block][row of its share][token]
   __shared__ __align__(8) uint64_t bars[2 * kSplitStages + 2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ __align__(16) float q_scales[NTOK];
   const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (kSplitStages + s); };
@@ -307,8 +327,9 @@ __global__ void __launch_bounds__(192, 2)
       mbar_init(empty(s), 1);
     }
     mbar_init(acc_full, 1);
-    mbar_init(sums_full, split * max(1, share / 32));           // a warp that sends arrives
+    mbar_init(sums_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    if (split > 1) mbar_expect_tx(sums_full, (uint32_t)((M + Cfg::kBlock - 1) / Cfg::kBlock * Cfg::kBlock) * 128u * 4u);       // what the cluster sends here
     pdl_launch_dependents();
     for (int kb = kb0; kb < kb1 && ahead < stages; ++kb, ++ahead) {
       mbar_expect_tx(full(ahead), kStage);
@@ -364,65 +385,67 @@ __global__ void __launch_bounds__(192, 2)
   // every thread of the cluster comes here, whatever its waits returned
   if (split > 1) cluster_wait();
   if (warp >= 2) {
-    const bool ok = mbar_wait_limited(acc_full, 0u, abortp, 4, error);
     // a lane of tensor memory is a row of w, a column a row of q
-    const int nl = (warp & 3) * 32 + lane, n = t * 128 + nl;
+    const int etid = threadIdx.x - 64, nl = (warp & 3) * 32 + lane, n = t * 128 + nl, n_mine = t * 128 + r * share + etid % share;
+    const float ws = split == 1 ? (n < N ? w_scale[n] : 0.f) : (n_mine < N ? w_scale[n_mine] : 0.f);
+    if (split > 1 && etid < M) q_scales[etid] = q_scale[etid];
+    const bool ok = mbar_wait_limited(acc_full, 0u, abortp, 4, error);
     const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const float ws = split == 1 && n < N ? w_scale[n] : 0.f;
-    const int owner = nl / share;
-    const uint32_t to = split > 1 ? remote_address(sums_base + (uint32_t)((r * share + nl % share) * kPitch) * 4u, owner) : 0u;
     tcgen05_fence_after();
+    if (split == 1) {
 #pragma unroll
-    for (int cb = 0; cb < NTOK; cb += 16) {
-      if (cb < M && ok) {
-        uint32_t v[16];
-        __syncwarp();
-        tcgen05_ld_32x32b_x16(taddr + cb, v);
-        if (split > 1) {
+      for (int cb = 0; cb < NTOK; cb += 16) {
+        if (cb < M && ok) {
+          uint32_t v[16];
+          __syncwarp();
+          tcgen05_ld_32x32b_x16(taddr + cb, v);
+          if (n < N) store_transposed<TOut>(out + (int64_t)cb * ldo + n, ldo, v, ws, q_scale + cb, M - cb);
+        }
+      }
+      tcgen05_fence_before();
+    } else {
+      const int rows = min(share, 32), owner = nl / share;
+      const uint32_t to = remote_address(sums_base + (uint32_t)(r * share * NTOK + nl % share * Cfg::kBlock) * 4u, owner), to_bar = remote_address(sums_full, owner);
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            if (cb + i < M) send_vec(to + (uint32_t)(cb + i) * 4u, v[i], v[i + 1], v[i + 2], v[i + 3]);
+      for (int cb = 0; cb < NTOK; cb += Cfg::kBlock) {
+        if (cb < M && ok) {
+          const uint32_t from = smem_base + 4u * 128u * cb;      // the stages are free: every product has been formed
+#pragma unroll
+          for (int h = 0; h < Cfg::kBlock; h += 16) {
+            uint32_t v[16];
+            __syncwarp();
+            tcgen05_ld_32x32b_x16(taddr + cb + h, v);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(from + 4u * sum_at<Cfg::kBlock>(nl, (h + i) / 4)), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]),
+                           "r"(v[i + 3])
+                           : "memory");
           }
-        } else if (n < N) {
-          store_transposed<TOut>(out + (int64_t)cb * ldo + n, ldo, v, ws, q_scale + cb, M - cb);
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          __syncwarp();
+          if (lane % rows == 0) send_bytes(to + 4u * cb * share, from + 4u * nl * Cfg::kBlock, 4u * rows * Cfg::kBlock, to_bar);
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      mbar_wait_limited<true>(sums_full, 0u, abortp, 5, error);
+      cluster_arrive();        // all that was sent here has come
+      asm volatile("bar.sync 1, 128;\n" ::: "memory");      // the rows' scales
+      if (n_mine < N) {
+        out += n_mine;
+        switch (split) {
+          case 2: add_share<TOut, 2, NTOK>(out, ldo, sums, q_scales, ws, M); break;
+          case 4: add_share<TOut, 4, NTOK>(out, ldo, sums, q_scales, ws, M); break;
+          default: add_share<TOut, 8, NTOK>(out, ldo, sums, q_scales, ws, M); break;
         }
       }
     }
-    tcgen05_fence_before();
-    if (split > 1) {
-      asm volatile("fence.acq_rel.cluster;\n" ::: "memory");
-      __syncwarp();
-      if (lane % share == 0) arrive_remote(remote_address(sums_full, owner));
-    }
+  } else if (split > 1) {
+    cluster_arrive();
   }
   if (split > 1) {
-    cluster_arrive();    // this CTA has sent all it has
-    if (warp >= 2) {
-      mbar_wait_limited<true>(sums_full, 0u, abortp, 5, error);
-      const int etid = threadIdx.x - 64, quads = (M + 3) / 4;
-      for (int i = etid; i < share * quads; i += 128) {
-        const int row = i % share, m = i / share * 4, n = t * 128 + r * share + row;
-        float4 part[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if (c < split) part[c] = *reinterpret_cast<const float4*>(sums + (c * share + row) * kPitch + m);
-        }
-        float4 sum = part[0];
-#pragma unroll
-        for (int c = 1; c < 8; ++c) {
-          if (c < split) sum.x += part[c].x, sum.y += part[c].y, sum.z += part[c].z, sum.w += part[c].w;
-        }
-        if (n < N) {
-          const float f = w_scale[n], o[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (m + j < M) out[(int64_t)(m + j) * ldo + n] = from_float<TOut>(o[j] * f * q_scale[m + j]);
-          }
-        }
-      }
-    }
     __syncwarp();
-    cluster_wait();      // nobody leaves before all that is sent to it has come
+    cluster_wait();      // nobody leaves before what it sends has arrived
   }
   let_copies_land(abortp);
   tcgen05_fence_before();
@@ -741,9 +764,9 @@ struct Operands {
 };
 
 // The few-row form: `split` CTAs a tile, as many (up to 8) as leave a processor one CTA, and two blocks of k for each: a processor's second CTA waits for
-// the same tensor cores, and the sums of a cluster cost more than it brings (8 x 4,096 x 4,096: split 4 6.6 us, 8 8.2, 2 8.3; 8 x 12,288 x 4,096:
-// 1 12.7, 2 14.1; 8 x 24,576 x 4,096: 1 19.6, 2 22.9).
-// At least `least`, where the sums ask for it.
+// the same tensor cores, and the sums of a cluster cost more than it brings (16 x 4,096 x 4,096: split 4 6.6 us, 8 8.0; 16 x 12,288 x 4,096:
+// 1 12.7, 2 14.8; 16 x 24,576 x 4,096: 1 19.1, 2 24.6). At least `least`, where the sums ask for it. (Clusters of three, for the 6,144 outputs of which
+// two leave a third of the processors alone, took 10.8 us for 9.1: 48 of them do not fit at once but where two share a processor.)
 int split_of(int64_t tiles, int k, int least = 1) {
   const int kbs = (k + kBlockK - 1) / kBlockK;
   int split = 8;
@@ -824,14 +847,15 @@ int launch_any(const Operands& o) {
 
 // The form with the least time by a count of its steps: rounds of tiles over the processors, a block of k each, and what a launch takes beside. A block of k
 // takes as long for 128 columns as for 64 (a product of 128 x 32 from shared memory takes 128 cycles up to there), 0.41 us for 256 and 0.37 for a
-// pair's 256 x 256, measured over 4,096 x 4,096 x 12,288 (385, 193, 155 and 143 us); beside it 512 rows x 4,096 x 4,096 took 3.7, 4.2, 4.1 and 4.4 us more.
+// pair's 256 x 256, measured over 4,096 x 4,096 x 12,288 (385, 193, 155 and 143 us); beside it 512 rows x 4,096 x 4,096 took 3.7, 4.2, 4.1 and 4.4 us more, and
+// the split form 7 to 8 (128 x 4,096 x 4,096 9.7 us for 8 blocks, 256 x 4,096 x 12,288 22.7 for 48).
 enum Form { kTile64, kTile128, kTile256, kPair, kSplit };
 Form form_of(int m, int n, int k) {
   const int64_t sms = processors(), kbs = (k + kBlockK - 1) / kBlockK;
   const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
   const float cost[5] = {up(up(m, 128) * up(n, 64), sms) * kbs * 0.272f + 3.7f, up(up(m, 128) * up(n, 128), sms) * kbs * 0.287f + 4.2f,
                          up(up(m, 128) * up(n, 256), sms) * kbs * 0.405f + 4.1f, up(up(m, 256) * up(n, 256), sms / 2) * kbs * 0.373f + 4.4f,
-                         up(up(m, 128) * up(n, 128) * split_of(up(m, 128) * up(n, 128), k), sms) * up(kbs, split_of(up(m, 128) * up(n, 128), k)) * 0.3f + 8.0f};
+                         up(up(m, 128) * up(n, 128) * split_of(up(m, 128) * up(n, 128), k), sms) * up(kbs, split_of(up(m, 128) * up(n, 128), k)) * 0.287f + 7.5f};
   int best = 0;
   for (int i = 1; i < 5; ++i) {
     if (cost[i] < cost[best]) best = i;
@@ -843,11 +867,11 @@ template <typename TOut>
 int launch_gemm(const Operands& o) {
   const bool tma = o.k % 16 == 0 && o.ldq % 16 == 0 && o.ldw % 16 == 0 && (uintptr_t)o.q % 16 == 0 && (uintptr_t)o.w % 16 == 0;
   if (!tma) return launch_any<TOut>(o);
-  // A handful of rows whose strips of w all run at once, two blocks a processor; one, where a warp asks more than once for its part of k. Against the
-  // split form: 8 x 4,096 x 4,096 5.7 us, 7.0; 8 x 1,024 x 4,096 4.3, 5.0; 8 x 2,000 x 16,000 14.5, 17.1; but 8 x 4,096 x 12,288 14.1, 12.1 and
-  // 8 x 24,576 x 4,096 25.8, 19.3.
+  // A handful of rows whose strips of w all run at once, two blocks a processor, with a k that the warps ask for at once. Against the split
+  // form: 8 x 4,096 x 4,096 5.7 us, 6.6; 8 x 2,048 x 2,048 3.7, 4.1; 8 x 512 x 2,048 2.6, 3.6; 8 x 1,024 x 4,096 4.2, 4.0; but 8 x 1,024 x 8,192
+  // 7.7, 5.6; 8 x 2,000 x 16,000 14.5, 12.0; 8 x 24,576 x 4,096 25.8, 19.2.
   const int strips = (o.n + 15) / 16;
-  if (o.m <= 8 && (strips <= processors() || (strips <= 2 * processors() && o.k <= 64 * 8 * kRowsDeep))) return launch_rows<TOut>(o);
+  if (o.m <= 8 && strips <= 2 * processors() && o.k <= kRowsMaxK) return launch_rows<TOut>(o);
   if (o.m <= 16) return launch_split<TOut, 16>(o);
   if (o.m <= 32) return launch_split<TOut, 32>(o);
   if (o.m <= 64) return launch_split<TOut, 64>(o);
