@@ -189,11 +189,12 @@ __device__ __forceinline__ void store_transposed(TOut* dst, int64_t ldo, const u
 }
 
 // ------------------------------------------------------------------------------------------------ a handful of rows
-// Latency is all there is to a product of up to 8 rows of q with a small w: a block takes 16 rows of w, its eight warps the blocks of 64 of k in turn,
-// straight from memory into the registers of mma.sync (m16n8k32): no barrier or copy engine lies between the loads and the products, and all of a
-// warp's blocks of w, kRowsDeep at most, are on their way before the wait for the kernel that makes q. A lane takes 16 numbers of a row at once; which k a
-// register of the instruction calls its own does not matter as long as both operands agree. The warps' sums meet in shared memory.
-constexpr int kRowsDeep = 8, kRowsMaxK = 64 * 8 * kRowsDeep;
+// Latency is all there is to a product of up to 16 rows of q with a small w: a block takes 16 rows of w, its eight warps the blocks of 64 of k in turn,
+// straight from memory into the registers of mma.sync (m16n8k32, NT times 8 rows of q): no barrier or copy engine lies between the loads and the products,
+// and all of a warp's blocks of w, up to DEEP, are on their way before the wait for the kernel that makes q (a loop over further ones cost 8 x 4,096 x
+// 4,096 0.9 us, blocks behind the end of k 8 x 4,096 x 1,024 0.4). A lane takes 16 numbers of a row at once; which k a register of the instruction calls
+// its own does not matter as long as both operands agree. The warps' sums meet in shared memory.
+constexpr int kRowsStep = 8 * 64;     // of k, by all warps once
 __device__ __forceinline__ void mma_e4m3_k32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -204,21 +205,21 @@ __device__ __forceinline__ uint4 load_stream(const uint8_t* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-template <typename TOut>
-__global__ void __launch_bounds__(256, 2)
+template <typename TOut, int NT, int DEEP>
+__global__ void __launch_bounds__(256, DEEP == 2 ? 4 : (DEEP == 4 && NT == 1 ? 3 : 2))
     gemm_e4m3_rows_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ w, const float* __restrict__ q_scale, const float* __restrict__ w_scale,
                           TOut* __restrict__ out, int M, int N, int K, int64_t ldq, int64_t ldw, int64_t ldo) {
-  __shared__ float part[8][8][17];
+  __shared__ float part[8][8 * NT][17];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int n0 = blockIdx.x * 16;
   const uint4 zero = make_uint4(0, 0, 0, 0);
   const uint8_t* w0 = w + (int64_t)min(n0 + g, N - 1) * ldw + 16 * c;
   const uint8_t* w1 = w + (int64_t)min(n0 + g + 8, N - 1) * ldw + 16 * c;
-  float acc[4] = {};
-  uint4 a[kRowsDeep][2];
+  float acc[NT][4] = {};
+  uint4 a[DEEP][2];
   pdl_launch_dependents();
 #pragma unroll
-  for (int i = 0; i < kRowsDeep; ++i) {
+  for (int i = 0; i < DEEP; ++i) {
     const int k = (warp + 8 * i) * 64;
     const bool in = k + 16 * c < K;
     a[i][0] = in ? load_stream(w0 + k) : zero;
@@ -226,29 +227,38 @@ __global__ void __launch_bounds__(256, 2)
   }
   pdl_wait();
 #pragma unroll
-  for (int i = 0; i < kRowsDeep; ++i) {
+  for (int i = 0; i < DEEP; ++i) {
     const int k = (warp + 8 * i) * 64 + 16 * c;
-    const uint4 b = g < M && k < K ? *reinterpret_cast<const uint4*>(q + (int64_t)g * ldq + k) : zero;
-    mma_e4m3_k32(acc, a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
-    mma_e4m3_k32(acc, a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
-  }
-  part[warp][2 * c][g] = acc[0];
-  part[warp][2 * c + 1][g] = acc[1];
-  part[warp][2 * c][g + 8] = acc[2];
-  part[warp][2 * c + 1][g + 8] = acc[3];
-  __syncthreads();
-  const int i = threadIdx.x, n = n0 + (i & 15), m = i >> 4;
-  if (m < M && n < N) {
-    float sum = part[0][m][i & 15];
 #pragma unroll
-    for (int v = 1; v < 8; ++v) sum += part[v][m][i & 15];
-    out[(int64_t)m * ldo + n] = from_float<TOut>(sum * w_scale[n] * q_scale[m]);
+    for (int t = 0; t < NT; ++t) {
+      const int m = 8 * t + g;
+      const uint4 b = m < M && k < K ? *reinterpret_cast<const uint4*>(q + (int64_t)m * ldq + k) : zero;
+      mma_e4m3_k32(acc[t], a[i][0].x, a[i][1].x, a[i][0].y, a[i][1].y, b.x, b.y);
+      mma_e4m3_k32(acc[t], a[i][0].z, a[i][1].z, a[i][0].w, a[i][1].w, b.z, b.w);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    part[warp][8 * t + 2 * c][g] = acc[t][0];
+    part[warp][8 * t + 2 * c + 1][g] = acc[t][1];
+    part[warp][8 * t + 2 * c][g + 8] = acc[t][2];
+    part[warp][8 * t + 2 * c + 1][g + 8] = acc[t][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 128 * NT; i += 256) {
+    const int n = n0 + (i & 15), m = i >> 4;
+    if (m < M && n < N) {
+      float sum = part[0][m][i & 15];
+#pragma unroll
+      for (int v = 1; v < 8; ++v) sum += part[v][m][i & 15];
+      out[(int64_t)m * ldo + n] = from_float<TOut>(sum * w_scale[n] * q_scale[m]);
+    }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
 // The weight's bytes are the time, so all that it takes is on its way at once: a cluster of `split` CTAs takes 128 rows of w, CTA r the r-th part of k,
-// two or three CTAs a processor, and every CTA asks for all its stages of w before it waits for the kernel that makes q. CTA o adds up the o-th part
+// and every CTA asks for all its stages of w before it waits for the kernel that makes q. CTA o adds up the o-th part
 // of the tile's rows: every CTA lays its sums into the stages, free by then, and a bulk copy a warp sends the rows of CTA o there, which counts the bytes
 // and adds the parts in CTA order.
 constexpr int kSplitStages = 8;
@@ -781,7 +791,7 @@ int launch_split(const Operands& o) {
   using Cfg = SplitCfg<NTOK>;
   const int tiles = (o.n + 127) / 128, chunks = (o.m + NTOK - 1) / NTOK, split = split_of((int64_t)tiles * chunks, o.k, two_chains<TOut>(o.k) ? 2 : 1);
   const int kbs = (o.k + kBlockK - 1) / kBlockK;
-  // Six stages, four for a short part of k (8 x 4,096 x 4,096: 6.6 us, 7.2 with six); where a processor has two CTAs, as many as let both in.
+  // Six stages, four for a short part of k (16 x 4,096 x 4,096: 6.6 us, 7.2 with six); where a processor has two CTAs, as many as let both in.
   const size_t sums = split > 1 ? Cfg::kSums : 0, room = ((int64_t)tiles * chunks * split > processors() ? 112 : 224) * 1024 - 1024 - sums;
   int stages = kbs / split <= 8 ? 4 : 6;
   while (stages > 2 && stages * (size_t)Cfg::kStage > room) --stages;
@@ -829,9 +839,9 @@ int launch_pair(const Operands& o) {
   return check_launch("gemm_e4m3 (pairs)");
 }
 
-template <typename TOut>
+template <typename TOut, int NT, int DEEP>
 int launch_rows(const Operands& o) {
-  launch_kernel(gemm_e4m3_rows_kernel<TOut>, dim3((o.n + 15) / 16), dim3(256), 0, o.stream, (const uint8_t*)o.q, (const uint8_t*)o.w, o.q_scale, o.w_scale,
+  launch_kernel(gemm_e4m3_rows_kernel<TOut, NT, DEEP>, dim3((o.n + 15) / 16), dim3(256), 0, o.stream, (const uint8_t*)o.q, (const uint8_t*)o.w, o.q_scale, o.w_scale,
                 (TOut*)o.out, o.m, o.n, o.k, o.ldq, o.ldw, o.ldo);
   return check_launch("gemm_e4m3 (a handful of rows)");
 }
@@ -867,11 +877,19 @@ template <typename TOut>
 int launch_gemm(const Operands& o) {
   const bool tma = o.k % 16 == 0 && o.ldq % 16 == 0 && o.ldw % 16 == 0 && (uintptr_t)o.q % 16 == 0 && (uintptr_t)o.w % 16 == 0;
   if (!tma) return launch_any<TOut>(o);
-  // A handful of rows whose strips of w all run at once, two blocks a processor, with a k that the warps ask for at once. Against the split
-  // form: 8 x 4,096 x 4,096 5.7 us, 6.6; 8 x 2,048 x 2,048 3.7, 4.1; 8 x 512 x 2,048 2.6, 3.6; 8 x 1,024 x 4,096 4.2, 4.0; but 8 x 1,024 x 8,192
-  // 7.7, 5.6; 8 x 2,000 x 16,000 14.5, 12.0; 8 x 24,576 x 4,096 25.8, 19.2.
-  const int strips = (o.n + 15) / 16;
-  if (o.m <= 8 && strips <= 2 * processors() && o.k <= kRowsMaxK) return launch_rows<TOut>(o);
+  // A handful of rows. Against the split form, us: 8 rows x 2,048 x 2,048 3.0, 4.1; x 512 x 2,048 1.8, 3.6; x 4,096 x 4,096 4.8, 6.6; x 6,144 x 4,096 7.5,
+  // 8.9; x 16,384 x 4,096 14.4, 14.4; x 24,576 x 2,048 11.2, 11.9; but x 24,576 x 4,096 19.8, 19.3 and x 32,768 x 512 6.2, 5.4. 16 rows x 4,096 x 4,096
+  // 5.8, 6.6; x 8,192 x 1,024 3.9, 4.7; but x 12,288 x 1,024 5.5, 5.2; x 8,192 x 2,048 7.6, 6.6; x 1,024 x 4,096 4.6, 4.0. A longer k, in several
+  // turns: 8 x 1,024 x 8,192 7.7, 5.4; 8 x 2,000 x 16,000 14.5, 12.0.
+  const int64_t strips = (o.n + 15) / 16, sms = processors();
+  if (o.k <= 8 * kRowsStep) {
+    if (o.m <= 8 && strips <= 11 * sms && (int64_t)o.n * o.k <= 1 << 26) {
+      return o.k <= 2 * kRowsStep ? launch_rows<TOut, 1, 2>(o) : (o.k <= 4 * kRowsStep ? launch_rows<TOut, 1, 4>(o) : launch_rows<TOut, 1, 8>(o));
+    }
+    if (o.m > 8 && o.m <= 16 && strips <= (o.k <= 2 * kRowsStep ? 4 : 2) * sms) {
+      return o.k <= 2 * kRowsStep ? launch_rows<TOut, 2, 2>(o) : (o.k <= 4 * kRowsStep ? launch_rows<TOut, 2, 4>(o) : launch_rows<TOut, 2, 8>(o));
+    }
+  }
   if (o.m <= 16) return launch_split<TOut, 16>(o);
   if (o.m <= 32) return launch_split<TOut, 32>(o);
   if (o.m <= 64) return launch_split<TOut, 64>(o);

@@ -168,6 +168,18 @@ def test_product(kernels, out, m, n, k):
     assert torch.equal(got, again), "the same bits on every run"
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(1, 17, 1024), (8, 300, 1040), (3, 2049, 1536), (8, 4100, 2032), (6, 15000, 1040), (7, 16300, 2048), (2, 12001, 4080), (8, 26100, 528),
+                                   (9, 33, 1024), (16, 9000, 528), (16, 9500, 1008), (11, 520, 2048), (13, 4700, 4096), (9, 100, 3600), (16, 4800, 2064), (10, 40000, 272)])
+def test_product_of_a_handful_of_rows(kernels, out, m, n, k):
+    """Both numbers of rows, the three depths of k with ends inside a block, strips that all run at once, that take turns, and one more than there are."""
+    q, q_scale = kernels.quantise_e4m3(rand((m, k), torch.float32, 8))
+    w, w_scale = kernels.quantise_e4m3(rand((n, k), torch.float32, 9, 0.02))
+    got = kernels.gemm_e4m3(q, q_scale, w, w_scale, out)
+    product_check(got, q, q_scale, w, w_scale, f"product {m} x {n} x {k}")
+    assert torch.equal(got, kernels.gemm_e4m3(q, q_scale, w, w_scale, out))
+
+
 @pytest.mark.parametrize("m,n,k", [(2, 5000, 12288), (7, 300, 8208), (30, 4100, 9008), (64, 20000, 8320), (90, 264, 16384), (300, 2050, 8208), (520, 4096, 8448),
                                    (1000, 4096, 14336), (2500, 4100, 8208), (4000, 72, 10240)])
 def test_product_of_a_long_k(kernels, m, n, k):
