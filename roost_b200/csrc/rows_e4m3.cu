@@ -474,7 +474,8 @@ static RowShape row_shape(int cols, int least_kv = 1) {
 static bool row_walk(int rows, int cols) { return cols > 8192 ? rows >= kFewRows : cols >= 4096 && (int64_t)rows * cols >= 1 << 24; }
 static bool whole16(const void* p) { return (uintptr_t)p % 16 == 0; }
 
-// The walk over many rows; false where a row has too many numbers for it. bytes: a row's inputs.
+// The walk over many rows; false where a ring of its rows does not fit in shared memory. bytes: a row's inputs.
+constexpr int kWalkSmem = 220 * 1024;      // what the kernel is allowed: with its barriers below the 227 KB that a block may have
 template <int KV, typename Source>
 static bool launch_walk(const Source& src, size_t bytes, uint8_t* q, float* scale, int rows, int cols, float eps, cudaStream_t stream) {
   int* error = gemm_tcgen05_error_address();
@@ -483,11 +484,11 @@ static bool launch_walk(const Source& src, size_t bytes, uint8_t* q, float* scal
   int stages = kRowStages;
   while (stages > 2 && stages * bytes > 32 * 1024) --stages;
   const size_t smem = stages * bytes;
+  if (!error || smem > kWalkSmem) return false;
   const int by_threads = 1024 / ((threads + 127) / 128 * 128), by_smem = (int)((224 * 1024) / (smem + 2048)), blocks = by_threads < by_smem ? by_threads : by_smem;
-  if (!error || blocks < 1) return false;
   auto kernel = rows_e4m3_walk_kernel<KV, Source>;
   static std::atomic<uint64_t> done{0};
-  if (smem > 40 * 1024) allow_smem(kernel, 220 * 1024, done);
+  if (smem > 40 * 1024) allow_smem(kernel, kWalkSmem, done);
   const int grid = blocks * processors();
   launch_kernel(kernel, dim3(rows < grid ? rows : grid), dim3(threads), smem, stream, src, q, scale, rows, cols, eps, stages, error);
   return true;
