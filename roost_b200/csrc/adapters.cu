@@ -742,7 +742,8 @@ extern "C" int roost_adapters_add(void* y, int64_t ldy, const void* x, int64_t l
   const size_t smem = (size_t)tile_rows * n_parts * rank * sizeof(float);
   ROOST_DISPATCH_DTYPE(dtype, T, ROOST_DISPATCH_DTYPE(y_dtype, TY, {
                          auto kernel = adapters_any_kernel<T, TY>;
-                         if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                         static std::atomic<uint64_t> done{0};
+                         if (smem > 40 * 1024) allow_smem(kernel, kAdapterTile * kAdapterMaxWidth * (int)sizeof(float), done);
                          launch_kernel(kernel, dim3(n_tiles * kAdapterCluster), dim3(kAdapterThreads), smem, (cudaStream_t)stream, (TY*)y, ldy, (const T*)x, ldx,
                                        (const T*)a, (const T*)b, scales, ranks, rows, tiles, tile_rows, tokens, listed, slots, parts, rank, inputs);
                        }));

@@ -455,6 +455,11 @@ __global__ void rms_norm_e4m3_kernel(const T* __restrict__ x, TR* residual, cons
 }
 
 static int row_smem(int cols) { return cols * (int)sizeof(float); }
+// ... of which a kernel is allowed the longest row's once: a limit set to every call's own would take another thread's from it.
+template <typename Kernel>
+static void allow_row(Kernel kernel, int cols, std::atomic<uint64_t>& done) {
+  if (row_smem(cols) > 40 * 1024) allow_smem(kernel, row_smem(ROOST_E4M3_MAX_COLS), done);
+}
 static int row_threads(int cols) { return cols >= 1024 ? 512 : (cols >= 256 ? 256 : 64); }
 
 // Threads of a row in registers and vectors of eight numbers a thread: one where 1,024 threads are enough (2,400 norms of 4,096 14.2 us, 17.1 and 22.2 with
@@ -511,7 +516,8 @@ extern "C" int roost_quantise_e4m3(const void* x, int64_t ldx, void* q, float* s
       launch_kernel(kernel, dim3(rows), dim3(shape.threads), 0, (cudaStream_t)stream, (const T*)x, ldx, (uint8_t*)q, scale, cols);
     } else {
       auto kernel = quantise_e4m3_kernel<T>;
-      if (row_smem(cols) > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, row_smem(cols));
+      static std::atomic<uint64_t> done{0};
+      allow_row(kernel, cols, done);
       launch_kernel(kernel, dim3(rows), dim3(row_threads(cols)), row_smem(cols), (cudaStream_t)stream, (const T*)x, ldx, (uint8_t*)q, scale, cols);
     }
   });
@@ -537,7 +543,8 @@ extern "C" int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tok
       launch_kernel(kernel, dim3(tokens), dim3(shape.threads), 0, (cudaStream_t)stream, (const T*)x, (uint8_t*)q, scale, inter, block, shift);
     } else {
       auto kernel = silu_mul_e4m3_kernel<T>;
-      if (row_smem(inter) > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, row_smem(inter));
+      static std::atomic<uint64_t> done{0};
+      allow_row(kernel, inter, done);
       launch_kernel(kernel, dim3(tokens), dim3(row_threads(inter)), row_smem(inter), (cudaStream_t)stream, (const T*)x, (uint8_t*)q, scale, inter, block);
     }
   });
@@ -561,7 +568,8 @@ static void launch_norm_e4m3(const void* x, void* residual, const void* w, void*
     launch_kernel(kernel, dim3(n_out), dim3(shape.threads), 0, stream, (const T*)x, (TR*)residual, w, (uint8_t*)q, scale, (T*)kept, rows, hidden, eps, wdtype);
   } else {
     auto kernel = rms_norm_e4m3_kernel<T, TR>;
-    if (row_smem(hidden) > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, row_smem(hidden));
+    static std::atomic<uint64_t> done{0};
+    allow_row(kernel, hidden, done);
     launch_kernel(kernel, dim3(n_out), dim3(row_threads(hidden)), row_smem(hidden), stream, (const T*)x, (TR*)residual, w, (uint8_t*)q, scale, (T*)kept, rows, hidden, eps,
                   wdtype);
   }
