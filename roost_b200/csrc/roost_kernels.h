@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define ROOST_ABI_VERSION 18
+#define ROOST_ABI_VERSION 19
 
 #define ROOST_OK 0
 #define ROOST_ERR_INVALID 1      /* an argument is out of range or inconsistent; nothing was launched */
@@ -633,6 +633,8 @@ int roost_head_gate_mul(void* x, const void* g, int64_t ld_g, int col, int token
 int roost_quantise_e4m3(const void* x, int64_t ldx, void* q, float* scale, int rows, int cols, int dtype, roost_stream_t stream);
 /* v = silu(gate) * up in 32 bits, x and block as roost_silu_mul. */
 int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tokens, int inter, int block, int dtype, roost_stream_t stream);
+/* The same, and v rounded once to x's type in kept [tokens, inter] (null: nothing is kept). */
+int roost_silu_mul_e4m3_kept(const void* x, void* q, float* scale, void* kept, int tokens, int inter, int block, int dtype, roost_stream_t stream);
 /* v = rms_norm(s) * w in 32 bits with s = x, or residual + x rounded to residual_dtype (that of x, or float32) where residual is not null; s
  * replaces residual unless `rows` gathers (as roost_add_rms_norm). kept (null, or of x's type): v as the norm without the 8 bits gives it. */
 int roost_rms_norm_e4m3(const void* x, void* residual, const void* w, void* q, float* scale, void* kept, const int32_t* rows, int n_out, int hidden,

@@ -83,13 +83,16 @@ template <typename T>
 struct GatedRow {
   const T* x;
   int inter, block;
+  T* kept;        // null: only the 8 bits are wanted
   static constexpr bool kNorm = false;
   __device__ __forceinline__ float load(int i, float&) const {
     const int64_t g_at = block ? (int64_t)(i / block) * 2 * block + i % block : i;
     const float g = to_float(x[g_at]), u = to_float(x[g_at + (block ? block : inter)]);
     return gated(g, u);
   }
-  __device__ __forceinline__ void keep(int, float) const {}
+  __device__ __forceinline__ void keep(int i, float v) const {
+    if (kept) kept[i] = from_float<T>(v);
+  }
 };
 template <typename T, typename TR>
 struct NormRow {
@@ -183,9 +186,11 @@ struct PlainVec {
   __device__ __forceinline__ void make(int, int, float&) {}
   __device__ __forceinline__ void keep(int, const float (&)[8]) const {}
 };
-template <typename T, int KV>
+// KEEP: the product goes to memory in x's type as well.
+template <typename T, int KV, bool KEEP>
 struct GatedVec {
   const T* x;
+  T* kept;
   int inter, block, shift;   // block = 1 << shift, or shift is negative
   static constexpr bool kNorm = false;
   float v[KV][8], up[KV][8];
@@ -199,7 +204,9 @@ struct GatedVec {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[k][e] = gated(v[k][e], up[k][e]);
   }
-  __device__ __forceinline__ void keep(int, const float (&)[8]) const {}
+  __device__ __forceinline__ void keep(int i, const float (&o)[8]) const {
+    if constexpr (KEEP) store8(kept + i, o);
+  }
 };
 // EARLY: few rows, the weights are in registers ahead of the wait.
 template <typename T, typename TR, int KV, bool ADD, bool EARLY>
@@ -345,17 +352,19 @@ __device__ __forceinline__ void rows_e4m3_walk(const Source& src, uint8_t* q, fl
   }
 }
 
-template <typename T, int KV>
+template <typename T, int KV, bool KEEP>
 struct GatedSource {
   const T* x;
+  T* kept;
   int inter, block, shift;
   __device__ __forceinline__ uint32_t a_bytes() const { return 2 * inter * (uint32_t)sizeof(T); }
   __device__ __forceinline__ uint32_t b_bytes() const { return 0; }
   __device__ __forceinline__ const void* a(int t) const { return x + (size_t)t * 2 * inter; }
   __device__ __forceinline__ const void* b(int) const { return nullptr; }
-  __device__ __forceinline__ GatedVec<T, KV> row(int, const unsigned char* a, const unsigned char*) const {
-    GatedVec<T, KV> r;
+  __device__ __forceinline__ GatedVec<T, KV, KEEP> row(int t, const unsigned char* a, const unsigned char*) const {
+    GatedVec<T, KV, KEEP> r;
     r.x = reinterpret_cast<const T*>(a);
+    r.kept = KEEP ? kept + (size_t)t * inter : nullptr;
     r.inter = inter;
     r.block = block;
     r.shift = shift;
@@ -400,12 +409,14 @@ __global__ void __launch_bounds__(1024) quantise_e4m3_vec_kernel(const T* __rest
   row_e4m3_vec<KV>(row, q + t * cols, scale + t, cols, 0.f);
   rows_are_written();
 }
-template <typename T, int KV>
-__global__ void __launch_bounds__(1024) silu_mul_e4m3_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, int inter, int block, int shift) {
+template <typename T, int KV, bool KEEP>
+__global__ void __launch_bounds__(1024) silu_mul_e4m3_vec_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, T* __restrict__ kept, int inter,
+                                                                 int block, int shift) {
   pdl_launch_dependents();
   const size_t t = blockIdx.x;
-  GatedVec<T, KV> row;
+  GatedVec<T, KV, KEEP> row;
   row.x = x + t * 2 * inter;
+  row.kept = KEEP ? kept + t * inter : nullptr;
   row.inter = inter;
   row.block = block;
   row.shift = shift;
@@ -436,12 +447,12 @@ __global__ void quantise_e4m3_kernel(const T* __restrict__ x, int64_t ldx, uint8
   rows_are_written();
 }
 template <typename T>
-__global__ void silu_mul_e4m3_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, int inter, int block) {
+__global__ void silu_mul_e4m3_kernel(const T* __restrict__ x, uint8_t* __restrict__ q, float* __restrict__ scale, T* __restrict__ kept, int inter, int block) {
   extern __shared__ float buf[];
   pdl_launch_dependents();
   pdl_wait();
   const size_t t = blockIdx.x;
-  row_e4m3(GatedRow<T>{x + t * 2 * inter, inter, block}, q + t * inter, scale + t, inter, 0.f, buf);
+  row_e4m3(GatedRow<T>{x + t * 2 * inter, inter, block, kept ? kept + t * inter : nullptr}, q + t * inter, scale + t, inter, 0.f, buf);
 }
 template <typename T, typename TR>
 __global__ void rms_norm_e4m3_kernel(const T* __restrict__ x, TR* residual, const void* __restrict__ w, uint8_t* __restrict__ q,
@@ -524,31 +535,44 @@ extern "C" int roost_quantise_e4m3(const void* x, int64_t ldx, void* q, float* s
   return check_launch("quantise_e4m3");
 }
 
-extern "C" int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tokens, int inter, int block, int dtype, roost_stream_t stream) {
+template <typename T, bool KEEP>
+static void launch_silu_mul_e4m3(const T* x, uint8_t* q, float* scale, T* kept, int tokens, int inter, int block, cudaStream_t stream) {
+  const RowShape shape = row_shape(inter);
+  int shift = -1;
+  for (int i = 3; i < 31; ++i) shift = block == 1 << i ? i : shift;
+  if (shape.kv && whole16(x) && whole16(kept) && (uintptr_t)q % 8 == 0) {
+    if (row_walk(tokens, inter) &&
+        launch_walk<4>(GatedSource<T, 4, KEEP>{x, kept, inter, block, shift}, 2 * inter * sizeof(T), q, scale, tokens, inter, 0.f, stream))
+      return;
+    auto kernel = shape.kv == 1 ? silu_mul_e4m3_vec_kernel<T, 1, KEEP> : (shape.kv == 2 ? silu_mul_e4m3_vec_kernel<T, 2, KEEP> : silu_mul_e4m3_vec_kernel<T, 4, KEEP>);
+    launch_kernel(kernel, dim3(tokens), dim3(shape.threads), 0, stream, x, q, scale, kept, inter, block, shift);
+  } else {
+    auto kernel = silu_mul_e4m3_kernel<T>;
+    static std::atomic<uint64_t> done{0};
+    allow_row(kernel, inter, done);
+    launch_kernel(kernel, dim3(tokens), dim3(row_threads(inter)), row_smem(inter), stream, x, q, scale, kept, inter, block);
+  }
+}
+
+extern "C" int roost_silu_mul_e4m3_kept(const void* x, void* q, float* scale, void* kept, int tokens, int inter, int block, int dtype, roost_stream_t stream) {
   ROOST_REQUIRE(tokens >= 0 && inter > 0, "silu_mul_e4m3: tokens and inter must be positive");
   ROOST_REQUIRE(block >= 0 && (block == 0 || (inter % block == 0 && block % 8 == 0)),
                 "silu_mul_e4m3: the interleave block must divide inter and be a multiple of 8");
   if (tokens == 0) return ROOST_OK;
   if (inter > ROOST_E4M3_MAX_COLS) return fail(ROOST_ERR_UNSUPPORTED, "silu_mul_e4m3: a row of more than 51168 elements does not fit in shared memory");
   ROOST_REQUIRE(x && q && scale, "silu_mul_e4m3: a pointer is null");
-  const RowShape shape = row_shape(inter);
-  int shift = -1;
-  for (int i = 3; i < 31; ++i) shift = block == 1 << i ? i : shift;
   ROOST_DISPATCH_DTYPE(dtype, T, {
-    if (shape.kv && whole16(x) && (uintptr_t)q % 8 == 0) {
-      if (row_walk(tokens, inter) && launch_walk<4>(GatedSource<T, 4>{(const T*)x, inter, block, shift}, 2 * inter * sizeof(T), (uint8_t*)q, scale, tokens, inter, 0.f,
-                                                    (cudaStream_t)stream))
-        return check_launch("silu_mul_e4m3");
-      auto kernel = shape.kv == 1 ? silu_mul_e4m3_vec_kernel<T, 1> : (shape.kv == 2 ? silu_mul_e4m3_vec_kernel<T, 2> : silu_mul_e4m3_vec_kernel<T, 4>);
-      launch_kernel(kernel, dim3(tokens), dim3(shape.threads), 0, (cudaStream_t)stream, (const T*)x, (uint8_t*)q, scale, inter, block, shift);
+    if (kept) {
+      launch_silu_mul_e4m3<T, true>((const T*)x, (uint8_t*)q, scale, (T*)kept, tokens, inter, block, (cudaStream_t)stream);
     } else {
-      auto kernel = silu_mul_e4m3_kernel<T>;
-      static std::atomic<uint64_t> done{0};
-      allow_row(kernel, inter, done);
-      launch_kernel(kernel, dim3(tokens), dim3(row_threads(inter)), row_smem(inter), (cudaStream_t)stream, (const T*)x, (uint8_t*)q, scale, inter, block);
+      launch_silu_mul_e4m3<T, false>((const T*)x, (uint8_t*)q, scale, nullptr, tokens, inter, block, (cudaStream_t)stream);
     }
   });
   return check_launch("silu_mul_e4m3");
+}
+
+extern "C" int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tokens, int inter, int block, int dtype, roost_stream_t stream) {
+  return roost_silu_mul_e4m3_kept(x, q, scale, nullptr, tokens, inter, block, dtype, stream);
 }
 
 template <typename T, typename TR, bool ADD>

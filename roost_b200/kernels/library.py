@@ -15,7 +15,7 @@ import torch
 
 from . import build
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 F32, BF16 = 0, 1
 E4M3 = torch.float8_e4m3fn
 GATE_FUNCTIONS = {"silu": 0, "gelu_tanh": 1, "clamped_swish": 2}   # the codes of csrc/roost_kernels.h
@@ -252,6 +252,7 @@ _SIGNATURES = {
     "roost_moe_combine": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "roost_quantise_e4m3": [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "roost_silu_mul_e4m3": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "roost_silu_mul_e4m3_kept": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
     "roost_rms_norm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p],
     "roost_gemm_e4m3": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
     "roost_adapters_workspace_bytes": [c_int, c_int, c_int, c_int, c_int],
@@ -465,16 +466,18 @@ class KernelLibrary:
         self._call("roost_quantise_e4m3", x.data_ptr(), x.stride(0) if T > 1 else W, q.data_ptr(), scale.data_ptr(), T, W, dtype_code(x.dtype), _stream_of(here))
         return q, scale
 
-    def silu_mul_e4m3(self, x: torch.Tensor, block: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
-        """(q, scale) of silu(gate) * up, which is not rounded before; x and ``block`` as ``silu_mul``."""
+    def silu_mul_e4m3(self, x: torch.Tensor, block: int = 0, keep: bool = False):
+        """(q, scale) of silu(gate) * up, which is not rounded before; x and ``block`` as ``silu_mul``. With ``keep`` the product in x's type as a
+        third result (what the adapters beside the next projection read)."""
         here = _need_here("silu_mul_e4m3", x)
         _need(x, "x")
         if x.dim() != 2 or x.shape[1] % 2:
             raise KernelError(f"silu_mul_e4m3: x is {tuple(x.shape)}; expected rows of gate and up values")
         T, inter = x.shape[0], x.shape[1] // 2
         q, scale = x.new_empty((T, inter), dtype=E4M3), x.new_empty(T, dtype=torch.float32)
-        self._call("roost_silu_mul_e4m3", x.data_ptr(), q.data_ptr(), scale.data_ptr(), T, inter, block, dtype_code(x.dtype), _stream_of(here))
-        return q, scale
+        kept = x.new_empty((T, inter)) if keep else None
+        self._call("roost_silu_mul_e4m3_kept", x.data_ptr(), q.data_ptr(), scale.data_ptr(), _ptr(kept), T, inter, block, dtype_code(x.dtype), _stream_of(here))
+        return (q, scale, kept) if keep else (q, scale)
 
     def _rms_norm_e4m3(self, x, residual, w, eps, rows, keep):
         here = _need_here("rms_norm_e4m3", x, residual, w, rows)

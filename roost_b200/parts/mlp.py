@@ -74,6 +74,8 @@ class GatedMlp(FeedForward):
         plan = getattr(batch, "adapters", None)
         if plan is not None and self.rt.adapters is not None:     # gate and up pass through memory, where their adapters join them
             y = self.gate_up(x, plan=plan)
+            if self.rt.e4m3:      # the same 8 bits as without a plan, and beside them what the adapters read
+                return self.down(E4m3Rows(*k.silu_mul_e4m3(y, keep=True)), plan=plan)
             return self.down(k.silu_mul(y) if self.spec.activation == "silu" else k.gated_act_mul(y, self.spec.activation, float(self.spec.limit)), plan=plan)
         if self.rt.e4m3:
             return self.down(E4m3Rows(*k.silu_mul_e4m3(self.gate_up(x))))

@@ -51,8 +51,9 @@ class FakeKernels:
         v = self.rms_norm(s.float(), w, eps, rows)
         return (*self._rows_e4m3(v), v.to(x.dtype)) if keep else self._rows_e4m3(v)
 
-    def silu_mul_e4m3(self, x, block=0):
-        return self._rows_e4m3(self.silu_mul(x.float(), block))
+    def silu_mul_e4m3(self, x, block=0, keep=False):
+        v = self.silu_mul(x.float(), block)
+        return (*self._rows_e4m3(v), v.to(x.dtype)) if keep else self._rows_e4m3(v)
 
     def adapters_add_(self, y, x, a, b, scale, plan, widths=None, ranks=None):
         widths = (y.shape[1],) if widths is None else widths
