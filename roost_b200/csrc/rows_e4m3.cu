@@ -32,11 +32,13 @@ __device__ __forceinline__ float over(float v, float scale, float inv) {
   const float r = v * inv;
   return fmaf(fmaf(-r, scale, v), inv, r);
 }
-// silu(g) u. 1 / (1 + exp(-g)) is within a unit in its last place: what the exact quotient would add lies nineteen bits below the 8-bit rounding.
+// silu(g) u. The reciprocal is within a unit in its last place, where a quotient would be within half of one: of 7.5e7 numbers 78 are not the one nearest to the
+// formula's, 76 with the quotient, which takes 57 us for 4,096 x 12,288. A quarter of 1 + exp(-g) stands for it, so that the reciprocal is a normal number (others
+// are given as zero) wherever the exponential is finite; that takes 49.9 us for 46.9.
 __device__ __forceinline__ float gated(float g, float u) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + expf(-g)));
-  return g * r * u;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(expf(-g), 0.25f, 0.25f)));
+  return g * r * (0.25f * u);
 }
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);

@@ -154,3 +154,17 @@ def test_walks_on_two_streams_and_in_graphs(kernels):
             graphs[i][0].replay()
         torch.cuda.synchronize()
         assert all(same(graphs[i][1], wants[turn + i]) for i in range(2))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,inter", [(5, 44), (5, 96), (2, 9000), (300, 12288)])
+def test_gates_far_below_zero_beside_large_values(kernels, dtype, tokens, inter):
+    """exp(-g) is up to 2^128 there, and its reciprocal less than the least normal number; the product with up is an ordinary number. Every form of the kernel."""
+    g = torch.linspace(-88.5, -84.0, inter, device="cuda").to(dtype)
+    u = torch.full((inter,), 3e38, device="cuda").to(dtype)
+    x = torch.cat([g, u]).repeat(tokens, 1).contiguous()
+    want = silu_of(x)
+    assert float(want.abs().min()) > 90
+    q, scale, kept = kernels.silu_mul_e4m3(x, keep=True)
+    check_rows(q, scale, want, 9 * HALF, "silu_mul")
+    assert bool(((kept.double() - want).abs() <= (9 * HALF + torch.finfo(dtype).eps / 2) * want.abs()).all())
