@@ -50,10 +50,11 @@ int roost_abi_version(void);
  * weight-streaming product its first loads of weights, while the kernel before it on the stream is finishing.
  * With it on, a kernel reads before it waits for the kernel in front: weights (norm weights, biases and slopes, the products'
  * weight matrices, rotations' inv_freq), index tables (positions, slot_mapping, token_row, the `rows` of the norms, the work lists
- * of the attention kernels, q_indptr, kv_lens, kv_indptr, kv_indices, the `slots` of states) and pages of the cache that hold only tokens
+ * of the attention kernels, q_indptr, kv_lens, kv_indptr, kv_indices, the `slots` of states, the adapters' `rows`, `tiles` and `ranks`), the
+ * adapters' a, b and `scales`, and pages of the cache that hold only tokens
  * of earlier steps. A caller must therefore not have those written by a kernel of this library that is still on its way: every one of
- * them lets the next begin at once, so that not only the kernel directly in front may be running when a table is read, but the ones
- * ahead of it as well. A copy, a memset or a kernel that is not this library's between the writer and the reader is enough;
+ * them but roost_quantise_e4m3 lets the next begin at once, so that not only the kernel directly in front may be running when a table is read, but the ones
+ * ahead of it as well. roost_quantise_e4m3 makes weights, so it lets the next begin when its rows and scales are written. A copy, a memset or a kernel that is not this library's between the writer and the reader is enough;
  * activations and the pages of the step's own tokens are read after the wait. */
 void roost_set_pdl(int on);
 /* Message of the last non-OK status on this thread. */
@@ -641,7 +642,8 @@ int roost_rms_norm_e4m3(const void* x, void* residual, const void* w, void* q, f
                         float eps, int dtype, int residual_dtype, int wdtype, roost_stream_t stream);
 
 /* ---- gemm_e4m3.cu ---- */
-/* out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k], 32-bit sums, any sizes and strides (in elements). */
+/* out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k], 32-bit sums, any sizes and strides (in elements). w is a weight in the sense of
+ * roost_set_pdl: rows of roost_quantise_e4m3 may be w at once, those of roost_rms_norm_e4m3 and roost_silu_mul_e4m3 after a copy of them; q may come from all. */
 int roost_gemm_e4m3(const void* q, const float* q_scale, const void* w, const float* w_scale, void* out, int m, int n, int k, int64_t ldq, int64_t ldw,
                     int64_t ldo, int out_dtype, roost_stream_t stream);
 

@@ -67,9 +67,11 @@ __device__ __forceinline__ void block_sum_top(float& sum, float& top_value, floa
   top_value = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nwarps ? scratch_top[lane] : 0u));
 }
 
-// A weight's rows may go straight into a product, which reads its weight ahead of its wait: the next kernel begins only when the rows are written.
+// A weight's rows may go straight into a product, which reads its weight ahead of its wait: the next kernel begins only when the rows are written, for its
+// loads and for its tensor copies, which are ordered behind ordinary stores by a fence of their own.
 __device__ __forceinline__ void rows_are_written() {
   __threadfence();
+  asm volatile("fence.proxy.async.global;\n" ::: "memory");
   __syncthreads();
   pdl_launch_dependents();
 }

@@ -512,7 +512,9 @@ class KernelLibrary:
         return self._rms_norm_e4m3(x, residual, w, eps, rows, keep)
 
     def gemm_e4m3(self, q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k] for rows in 8 bits on either side (``quantise_e4m3`` and its like), 32-bit sums."""
+        """out[m, n] = q_scale[m] w_scale[n] sum_k q[m, k] w[n, k] for rows in 8 bits on either side, 32-bit sums. q: from ``quantise_e4m3``, the norms or
+        ``silu_mul_e4m3``. w is read while the kernel in front is still running: a weight at rest, or rows that ``quantise_e4m3`` has just made; rows of the
+        norms and of ``silu_mul_e4m3`` only as a copy (``w.clone()``)."""
         here = _need_here("gemm_e4m3", q, q_scale, w, w_scale)
         _need_rows(q, "q", E4M3); _need_rows(w, "w", E4M3)
         _need(q_scale, "q_scale", torch.float32); _need(w_scale, "w_scale", torch.float32)
