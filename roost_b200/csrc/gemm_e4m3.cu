@@ -719,7 +719,8 @@ __global__ void __launch_bounds__(256) gemm_e4m3_any_kernel(const uint8_t* __res
   pdl_launch_dependents();
   pdl_wait();
   const int n0 = blockIdx.x * kAnyTile, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int m0 = blockIdx.y * kAnyTile; m0 < M; m0 += gridDim.y * kAnyTile) {
+  for (int64_t at = blockIdx.y * kAnyTile; at < M; at += gridDim.y * kAnyTile) {     // 64 bits: one step behind the last rows may be beyond 32
+    const int m0 = (int)at;
     float acc[4][4] = {};
     for (int k0 = 0; k0 < K; k0 += kAnyK) {
       __syncthreads();
