@@ -42,6 +42,24 @@ __device__ __forceinline__ float adapter_load(uint32_t addr) {
 }
 __device__ __forceinline__ void adapter_store(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(addr), "f"(v) : "memory"); }
 
+struct AdapterTile {
+  int slot, first, rows, rank;   // rank 0: nothing to do
+};
+// A tile of the list, its range cut to the list whatever numbers it has.
+__device__ __forceinline__ AdapterTile adapter_tile(const int32_t* tiles, int tile, const int32_t* ranks, int tile_rows, int listed, int slots, int R) {
+  AdapterTile t;
+  t.slot = tiles[3 * tile];
+  t.first = max(tiles[3 * tile + 1], 0);
+  t.rows = min(min(max(tiles[3 * tile + 2], 0), listed) - t.first, tile_rows);
+  const bool empty = t.slot < 0 || t.slot >= slots || t.rows <= 0;
+  t.rank = empty ? 0 : (ranks ? min(max(ranks[t.slot], 0), R) : R);
+  return t;
+}
+__device__ __forceinline__ int adapter_row(const int32_t* rows, int at, int tokens) {
+  const int r = rows[at];
+  return r >= 0 && r < tokens ? r : -1;
+}
+
 // Adds up the eight CTAs' partial sums h[0 .. count) and leaves the sums, times `factor`, in every CTA: entry e is read and written by one CTA only,
 // the one that owns it, so the sums replace the parts in place.
 __device__ __forceinline__ void adapter_join(float* h, int count, float factor) {
@@ -77,13 +95,10 @@ __global__ void __launch_bounds__(kAdapterThreads) __cluster_dims__(kAdapterClus
   pdl_launch_dependents();
   pdl_wait();
   const int tile = blockIdx.x / kAdapterCluster, c = (int)adapter_cluster_rank();
-  const int slot = tiles[3 * tile], first = max(tiles[3 * tile + 1], 0), end = min(min(tiles[3 * tile + 2], listed), first + tile_rows);
-  if (slot < 0 || slot >= slots || end <= first) return;   // the whole cluster
-  const int n_rows = end - first, r_used = ranks ? min(max(ranks[slot], 0), R) : R, wide = parts.n * r_used;
-  for (int i = threadIdx.x; i < n_rows; i += kAdapterThreads) {
-    const int r = rows[first + i];
-    row_of[i] = r >= 0 && r < tokens ? r : -1;
-  }
+  const AdapterTile at_tile = adapter_tile(tiles, tile, ranks, tile_rows, listed, slots, R);
+  if (at_tile.rank == 0) return;   // the whole cluster
+  const int slot = at_tile.slot, n_rows = at_tile.rows, r_used = at_tile.rank, wide = parts.n * r_used;
+  for (int i = threadIdx.x; i < n_rows; i += kAdapterThreads) row_of[i] = adapter_row(rows, at_tile.first + i, tokens);
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int k0 = (int)((int64_t)K * c / kAdapterCluster), k1 = (int)((int64_t)K * (c + 1) / kAdapterCluster);
@@ -169,23 +184,6 @@ __device__ __forceinline__ void adapter_queue16(uint32_t smem, const void* gmem,
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem), "l"(gmem), "r"(in ? 16 : 0) : "memory");   // zeros where there is nothing
 }
 
-struct AdapterTile {
-  int slot, first, rows, rank;   // rank 0: nothing to do
-};
-__device__ __forceinline__ AdapterTile adapter_tile(const int32_t* tiles, int tile, const int32_t* ranks, int tile_rows, int listed, int slots, int R) {
-  AdapterTile t;
-  t.slot = tiles[3 * tile];
-  t.first = max(tiles[3 * tile + 1], 0);
-  t.rows = min(min(tiles[3 * tile + 2], listed) - t.first, tile_rows);
-  const bool empty = t.slot < 0 || t.slot >= slots || t.rows <= 0;
-  t.rank = empty ? 0 : (ranks ? min(max(ranks[t.slot], 0), R) : R);
-  return t;
-}
-__device__ __forceinline__ int adapter_row(const int32_t* rows, int at, int tokens) {
-  const int r = rows[at];
-  return r >= 0 && r < tokens ? r : -1;
-}
-
 // A cluster of `ctas` takes a tile of up to MT * 16 tokens, CTA v the v-th part of k, SK of k a stage: x's and a's rows by cp.async, whole lines of memory,
 // into swizzled rows of shared memory, as many stages as fit on their way, a's first ones ahead of the wait for x. Where all of a CTA's blocks fit
 // there is one wait for all of them. A thread copies the same pieces of the same rows in every stage, so that its addresses stay in registers. Warps: KG
@@ -216,13 +214,13 @@ template <int SPLIT, int MT, int KG, int NS, int NP, int SK>
 __global__ void __launch_bounds__(DownCfg<MT, KG, NS, NP, SK>::kThreads, DownCfg<MT, KG, NS, NP, SK>::kCtas)
     adapters_down_kernel(__nv_bfloat16* __restrict__ h_out, const __nv_bfloat16* __restrict__ x, int64_t ldx, const __nv_bfloat16* __restrict__ a,
                          const float* __restrict__ scales, const int32_t* __restrict__ ranks, const int32_t* __restrict__ rows, const int32_t* __restrict__ tiles,
-                         int tokens, int listed, int slots, int parts, int R, int K, int ctas, int stages, int stage_bytes) {
+                         int tile_rows, int tokens, int listed, int slots, int parts, int R, int K, int ctas, int stages, int stage_bytes) {
   using Cfg = DownCfg<MT, KG, NS, NP, SK>;
   constexpr int kRowsX = Cfg::kRowsX, kThreads = Cfg::kThreads, kWarps = Cfg::kWarps, kMw = Cfg::kMw, kPasses = Cfg::kPasses;
   extern __shared__ __align__(1024) unsigned char smem[];
   pdl_launch_dependents();
   const int cta = (int)adapter_cluster_rank();
-  const AdapterTile at = adapter_tile(tiles, blockIdx.x / ctas, ranks, kRowsX, listed, slots, R);
+  const AdapterTile at = adapter_tile(tiles, blockIdx.x / ctas, ranks, tile_rows, listed, slots, R);
   if (at.rank == 0) {    // the whole cluster
     pdl_wait();
     return;
@@ -624,8 +622,8 @@ static void launch_adapters_down(const AdapterCall& q) {
   auto kernel = adapters_down_kernel<SPLIT, MT, KG, NS, NP, SK>;
   static std::atomic<uint64_t> done{0};
   if (smem > 40 * 1024) allow_smem(kernel, 220 * 1024, done);
-  launch_kernel_cluster(kernel, dim3(q.n_tiles * ctas), dim3(Cfg::kThreads), smem, q.stream, ctas, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tokens,
-                        q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas, stages, stage);
+  launch_kernel_cluster(kernel, dim3(q.n_tiles * ctas), dim3(Cfg::kThreads), smem, q.stream, ctas, q.h, q.x, q.ldx, q.a, q.scales, q.ranks, q.rows, q.tiles, q.tile_rows,
+                        q.tokens, q.listed, q.slots, q.parts.n, q.rank, q.inputs, ctas, stages, stage);
 }
 template <typename TY, int SPLIT, int MT, int RB>
 static void launch_adapters_up(const AdapterCall& q) {
