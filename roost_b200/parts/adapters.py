@@ -28,9 +28,10 @@ class ProjectionAdapters:
     a: torch.Tensor          # [slots, parts, rank, in]
     b: torch.Tensor          # [slots, out, rank]
     widths: tuple
+    ranks: torch.Tensor      # [slots]: the adapters' ranks here; 0 where an adapter names no part of this projection, so that its tokens' rows are not touched
 
     def add_(self, y: torch.Tensor, x: torch.Tensor, plan) -> torch.Tensor:
-        return self.slots.kernels.adapters_add_(y, x, self.a, self.b, self.slots.scale, plan, widths=self.widths, ranks=self.slots.ranks)
+        return self.slots.kernels.adapters_add_(y, x, self.a, self.b, self.slots.scale, plan, widths=self.widths, ranks=self.ranks)
 
 
 class AdapterSlots:
@@ -51,8 +52,9 @@ class AdapterSlots:
             raise ValueError(f"adapters: parts {widths} are not the {out_features} outputs of the projection")
         if len(widths) * self.rank > MAX_PARTS_RANK:
             raise ValueError(f"adapters: rank {self.rank} beside a projection of {len(widths)} parts is beyond {MAX_PARTS_RANK // len(widths)}")
-        zeros = lambda *shape: torch.zeros(shape, dtype=self.dtype, device=self.device)
-        return ProjectionAdapters(self, zeros(self.count, len(widths), self.rank, in_features), zeros(self.count, out_features, self.rank), widths)
+        zeros = lambda *shape, dtype=self.dtype: torch.zeros(shape, dtype=dtype, device=self.device)   # noqa: E731
+        return ProjectionAdapters(self, zeros(self.count, len(widths), self.rank, in_features), zeros(self.count, out_features, self.rank), widths,
+                                  zeros(self.count, dtype=torch.int32))
 
     def free_slot(self) -> int:
         for s in range(self.count):
@@ -120,6 +122,9 @@ def place_adapter(slots: AdapterSlots, projections: dict, name, modules: dict, s
         else:
             pool.a[slot, part].zero_()
             pool.b[slot, rows].zero_()
+    named = {id(projections[module][0]) for module in modules}
+    for pool, _ in projections.values():
+        pool.ranks[slot] = rank if id(pool) in named else 0
     slots.scale[slot] = scale
     slots.ranks[slot] = rank
     slots.names[name] = slot
