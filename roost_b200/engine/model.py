@@ -46,6 +46,8 @@ class Model:
         # what each run keeps between steps (None: nothing, or another run's cache)
         self.cache_needs = []
         self.embedding_need = self.embedding.cache_need()
+        if runtime.adapters is not None:     # projections inside a part (a branch of a parallel mixer) have no name that an adapter could give
+            runtime.adapters.keep_only([pool for pool, _ in self.adapter_projections().values()])
         if runtime.e4m3:
             for i, b in enumerate(self.blocks):
                 for name, part in {"block": b, **b.sub_parts()}.items():

@@ -45,6 +45,7 @@ class AdapterSlots:
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
         self.names: dict = {}        # adapter -> slot
+        self.beside: list = []       # the projections that were given room since ``keep_only``
 
     def projection(self, out_features: int, in_features: int, widths: tuple | None = None) -> ProjectionAdapters:
         widths = (out_features,) if widths is None else tuple(widths)
@@ -55,6 +56,14 @@ class AdapterSlots:
         zeros = lambda *shape, dtype=self.dtype: torch.zeros(shape, dtype=dtype, device=self.device)   # noqa: E731
         return ProjectionAdapters(self, zeros(self.count, len(widths), self.rank, in_features), zeros(self.count, out_features, self.rank), widths,
                                   zeros(self.count, dtype=torch.int32))
+
+    def keep_only(self, pools: list) -> None:
+        """Takes the room back from the projections whose ``ProjectionAdapters`` are not among ``pools``: no adapter can be loaded there."""
+        kept = {id(p) for p in pools}
+        for part in self.beside:
+            if id(part.adapters) not in kept:
+                part.adapters = None
+        self.beside = []
 
     def free_slot(self) -> int:
         for s in range(self.count):

@@ -137,12 +137,13 @@ class E4m3Linear:
         return part
 
 
-def projection(runtime: Runtime, out_features: int, in_features: int, widths: tuple | None = None):
+def projection(runtime: Runtime, out_features: int, in_features: int, widths: tuple | None = None, adapters: bool = True):
     """A layer's projection without a bias, in the form ``Runtime.weights`` asks for, with room for adapters where the model has it (``widths``: the
-    parts of its outputs that have adapters of their own)."""
+    parts of its outputs that have adapters of their own) and ``adapters`` is true."""
     part = (E4m3Linear if runtime.e4m3 else Linear)(runtime, out_features, in_features)
-    if runtime.adapters is not None:
+    if runtime.adapters is not None and adapters:
         part.adapters = runtime.adapters.projection(out_features, in_features, widths)
+        runtime.adapters.beside.append(part)
     return part
 
 

@@ -18,7 +18,8 @@ GATE_FUNCTIONS = ("silu", "gelu_tanh", "clamped_swish")
 class GatedMlp(FeedForward):
     serves_e4m3 = True
 
-    def __init__(self, spec: GatedMlpSpec, runtime: Runtime):
+    def __init__(self, spec: GatedMlpSpec, runtime: Runtime, adapters: bool = True):
+        """``adapters``: whether the projections have room for adapters where the model has it."""
         if spec.hidden <= 0 or spec.intermediate <= 0:
             raise ValueError("gated_mlp: hidden and intermediate must be positive")
         if spec.activation not in GATE_FUNCTIONS:
@@ -29,14 +30,15 @@ class GatedMlp(FeedForward):
         self.rt = runtime
         if runtime.e4m3 and spec.activation != "silu":
             raise ValueError(f"gated_mlp: weights in e4m3 serve the activation 'silu', not '{spec.activation}'")
-        self.gate_up = projection(runtime, 2 * spec.intermediate, spec.hidden, (spec.intermediate, spec.intermediate))
-        self.down = projection(runtime, spec.hidden, spec.intermediate)
+        self.gate_up = projection(runtime, 2 * spec.intermediate, spec.hidden, (spec.intermediate, spec.intermediate), adapters)
+        self.down = projection(runtime, spec.hidden, spec.intermediate, adapters=adapters)
         # In bfloat16 with an intermediate size that is a multiple of 128 the gate and up rows are stored interleaved in
         # blocks of 128, the layout in which the tensor-core product applies SiLU(gate) * up to its accumulator, so that
         # for many rows of x the [T, 2I] product never goes to memory; few rows keep the library product and the
         # SiLU kernel, which reads the same layout.
         k = runtime.kernels
-        self.interleave = 128 if (not runtime.full_precision and not runtime.e4m3 and runtime.adapters is None and spec.intermediate % 128 == 0 and spec.hidden % 8 == 0
+        # Adapters take gate and up as two parts one behind the other, so a layer with room for them keeps that order and the two kernels.
+        self.interleave = 128 if (not runtime.full_precision and not runtime.e4m3 and self.gate_up.adapters is None and spec.intermediate % 128 == 0 and spec.hidden % 8 == 0
                                   and spec.activation == "silu" and hasattr(k, "gemm_tcgen05_swiglu")) else 0
         self.fused_min_rows = 256   # below this the 128-row tiles are mostly empty and the library product is faster
         # ... and so it is while the product is small: measured on a B200, the library product followed by the SiLU kernel
@@ -72,7 +74,7 @@ class GatedMlp(FeedForward):
     def __call__(self, x, batch=None):
         k = self.rt.kernels
         plan = getattr(batch, "adapters", None)
-        if plan is not None and self.rt.adapters is not None:     # gate and up pass through memory, where their adapters join them
+        if plan is not None and self.gate_up.adapters is not None:     # gate and up pass through memory, where their adapters join them
             y = self.gate_up(x, plan=plan)
             if self.rt.e4m3:      # the same 8 bits as without a plan, and beside them what the adapters read
                 return self.down(E4m3Rows(*k.silu_mul_e4m3(y, keep=True)), plan=plan)

@@ -70,7 +70,7 @@ class RoutedMlp(FeedForward):
         self.interleave = 128 if (not runtime.full_precision and s.expert_intermediate % 128 == 0 and s.hidden % 8 == 0
                                   and hasattr(runtime.kernels, "_moe_gemm_tcgen05")) else 0
         self.shared = (GatedMlp(GatedMlpSpec(hidden=s.hidden, intermediate=s.shared_intermediate, activation=s.activation,
-                                             limit=s.shared_limit), runtime) if s.shared_intermediate else None)
+                                             limit=s.shared_limit), runtime, adapters=False) if s.shared_intermediate else None)
 
     @classmethod
     def parameters(cls, spec: RoutedMlpSpec):

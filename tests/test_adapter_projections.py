@@ -56,3 +56,33 @@ def test_rows_of_a_projection_that_is_not_named_keep_their_bits(kernels, tiny_mo
         x = torch.randn((9, proj.in_features), generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
         proj.adapters.add_(y, x, kernels.adapter_plan([9], [slot]))
         assert bool(torch.signbit(y).all() and not y.any()) != touched
+
+
+def test_no_room_where_no_adapter_can_be_loaded(tiny_model_dirs, tmp_path):
+    """A shared expert beside routed ones and the branches of a parallel mixer have no module that an adapter could name: they keep no room, a step with
+    adapters runs nothing beside them, and a shared expert keeps the layout of its fused products."""
+    import dataclasses
+
+    from roost_b200.config.spec import ParallelMixerSpec, RoutedMlpSpec
+    from roost_b200.engine.model import Model
+    from roost_b200.parts import Runtime
+    from roost_b200.parts.routed_mlp import RoutedMlp
+
+    class Fused(FakeKernels):
+        gemm_tcgen05_swiglu = None     # that the fused product exists is what chooses the layout
+
+    spec = RoutedMlpSpec(hidden=64, experts=4, top=1, expert_intermediate=16, shared_intermediate=128)
+    with_room = RoutedMlp(spec, Runtime(torch.bfloat16, "cpu", Fused(), adapters=(2, 8))).shared
+    assert with_room.gate_up.adapters is None and with_room.down.adapters is None
+    assert with_room.interleave == RoutedMlp(spec, Runtime(torch.bfloat16, "cpu", Fused())).shared.interleave == 128
+
+    base = load_model(tiny_model_dirs["A"], torch.float32, "cpu", FakeKernels()).spec
+    blocks = [dataclasses.replace(b, mixer=ParallelMixerSpec(hidden=64, branches=(b.mixer, b.mixer))) if i == 0 else b for i, b in enumerate(base.blocks)]
+    names = {k: v for k, v in base.weight_names.items() if k != "blocks.0.mixer"}
+    names["blocks.0.mixer"] = {f"{n}.{local}": t for n in range(2) for local, t in base.weight_names["blocks.0.mixer"].items()}
+    model = Model(dataclasses.replace(base, blocks=blocks, weight_names=names), Runtime(torch.float32, "cpu", FakeKernels(), adapters=(2, 8)))
+    branches = model.blocks[0].mixer.branches
+    assert all(b.qkv.adapters is None and b.out.adapters is None for b in branches)
+    loadable = {id(p) for p, _ in model.adapter_projections().values()}
+    others = [model.blocks[0].feed_forward.gate_up, model.blocks[1].mixer.qkv, model.blocks[1].mixer.out, model.blocks[1].feed_forward.down]
+    assert all(id(p.adapters) in loadable for p in others)
