@@ -296,6 +296,7 @@ class AdapterPlan:
     tile_rows: int = 64      # tokens of a tile at most
 
 
+_INT_MAX = 2 ** 31 - 1
 ADAPTER_TILE_ROWS = 64       # tokens of a tile of an adapter plan at most
 ADAPTER_FEW_ROWS = 16        # ... where tiles of this many still leave processors without work
 ADAPTER_FEW_TILES = 37
@@ -306,9 +307,14 @@ def adapter_lists(row_counts: list, row_slots: list, tile_rows: int | None = Non
     adapter in slot ``row_slots[i]`` (negative: none). ``tile_rows``: the most tokens of a tile; None: chosen by the lists."""
     if len(row_counts) != len(row_slots):
         raise KernelError(f"adapter_plan: {len(row_counts)} requests, {len(row_slots)} adapters")
-    counts, slots = np.asarray(row_counts, np.int64), np.asarray(row_slots, np.int64)
-    if counts.size and counts.min() < 0:
-        raise KernelError("adapter_plan: a request has fewer than no tokens")
+    counts, slots = np.asarray(row_counts), np.asarray(row_slots)
+    if counts.size and (counts.dtype.kind not in "iu" or slots.dtype.kind not in "iu"):
+        raise KernelError("adapter_plan: numbers of tokens and slots are whole numbers")
+    if counts.size and (counts.min() < 0 or counts.max() > _INT_MAX or counts.sum(dtype=np.float64) > _INT_MAX):
+        raise KernelError("adapter_plan: a request has fewer than no tokens, or the step more than an index holds")
+    if slots.size and slots.max() > _INT_MAX:
+        raise KernelError(f"adapter_plan: slot {int(slots.max())} is more than an index holds")
+    counts, slots = counts.astype(np.int64), slots.astype(np.int64)
     of = np.repeat(slots, counts)                                   # each token's adapter
     order = np.argsort(of, kind="stable")
     rows = order[np.searchsorted(of[order], 0):]                    # tokens without an adapter are left out
