@@ -14,6 +14,7 @@ from pathlib import Path
 
 import torch
 
+OTHER_BASE = ("pissa", "olora", "corda", "loftq", "lora_ga")     # ways to begin an adapter that take something out of the base's weights
 MAX_PARTS_RANK = 512     # parts times rank that a projection's adapters may have
 
 
@@ -81,9 +82,16 @@ def read_adapter(folder) -> tuple[dict, float]:
         rank, alpha = int(config["r"]), float(config.get("lora_alpha", config["r"]))
     except (OSError, ValueError, KeyError, TypeError) as e:
         raise AdapterError(f"{folder}: adapter_config.json cannot be read ({e})") from None
-    for key in ("use_dora", "modules_to_save", "rank_pattern", "alpha_pattern"):
+    if str(config.get("peft_type", "LORA")).upper() != "LORA":
+        raise AdapterError(f"{folder}: adapters of type {config['peft_type']!r} are not served")
+    for key in ("use_dora", "modules_to_save", "rank_pattern", "alpha_pattern", "layer_replication", "alora_invocation_tokens", "use_qalora"):
         if config.get(key):
             raise AdapterError(f"{folder}: adapter_config.json asks for {key}, which is not served")
+    if str(config.get("init_lora_weights", "")).lower().startswith(OTHER_BASE):
+        raise AdapterError(f"{folder}: an adapter of init_lora_weights {config['init_lora_weights']!r} stands beside a base whose weights were changed with it; "
+                           "save it converted to the stored base")
+    if not math.isfinite(alpha):
+        raise AdapterError(f"{folder}: lora_alpha {alpha} is not finite")
     if config.get("bias", "none") != "none":
         raise AdapterError(f"{folder}: adapters with biases are not served")
     if rank <= 0:
