@@ -306,15 +306,16 @@ __device__ __forceinline__ void row_e4m3_vec(Row row, uint8_t* q, float* scale_o
   row_to_e4m3<KV, false>(row, q, scale_out, cols, eps, scratch, scratch_top, [] {});
 }
 
-// Many rows: a block walks rows gridDim apart. One thread asks for whole rows by bulk copies into a ring of `stages` rows of shared memory, so that the next
-// rows are on their way while this one is searched, rounded and stored; the exchange over the block is also where the row's place in the ring becomes
-// free. `Source` says what a row consists of: up to two ranges of memory, and its Row over their copies.
-constexpr int kRowStages = 4;
+// Many rows: a block walks rows gridDim apart. One thread asks for whole rows by bulk copies into a ring of two rows of shared memory, so that the next
+// row is on its way while this one is searched, rounded and stored; the exchange over the block is also where the row's place in the ring becomes
+// free (four rows, so fewer blocks a processor, took 8,192 norms of 4,096 from 45 us to 56). `Source` says what a row consists of: up to two ranges of memory,
+// and its Row over their copies.
+constexpr int kRowStages = 2;
 __device__ __forceinline__ void bulk_row(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 template <int KV, typename Source>
-__device__ __forceinline__ void rows_e4m3_walk(const Source& src, uint8_t* q, float* scale_out, int rows, int cols, float eps, int stages, int* error) {
+__device__ __forceinline__ void rows_e4m3_walk(const Source& src, uint8_t* q, float* scale_out, int rows, int cols, float eps, int* error) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ __align__(8) uint64_t bars[kRowStages];
   __shared__ float scratch[2][32];
@@ -330,14 +331,14 @@ __device__ __forceinline__ void rows_e4m3_walk(const Source& src, uint8_t* q, fl
   };
   if (threadIdx.x == 0) {
     abort_flag = 0;
-    for (int i = 0; i < stages; ++i) mbar_init(bar0 + 8u * i, 1);
+    for (int i = 0; i < kRowStages; ++i) mbar_init(bar0 + 8u * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
   pdl_launch_dependents();
   pdl_wait();
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 0; i < stages && blockIdx.x + i * gridDim.x < rows; ++i) ask(blockIdx.x + i * gridDim.x, i);
+    for (int i = 0; i < kRowStages && blockIdx.x + i * gridDim.x < rows; ++i) ask(blockIdx.x + i * gridDim.x, i);
   }
   int stage = 0, turn = 0;
   uint32_t phase = 0;
@@ -345,10 +346,10 @@ __device__ __forceinline__ void rows_e4m3_walk(const Source& src, uint8_t* q, fl
     mbar_wait_limited(bar0 + 8u * stage, phase, &abort_flag, 8, error);
     auto row = src.row(t, ring + (size_t)stage * bytes, ring + (size_t)stage * bytes + a_bytes);
     row_to_e4m3<KV, true>(row, q + (size_t)t * cols, scale_out + t, cols, eps, scratch[turn], scratch_top[turn], [&] {
-      const int next = t + stages * (int)gridDim.x;
+      const int next = t + kRowStages * (int)gridDim.x;
       if (threadIdx.x == 0 && next < rows && next > t) ask(next, stage);    // every thread has read this row
     });
-    if (++stage == stages) stage = 0, phase ^= 1u;
+    if (++stage == kRowStages) stage = 0, phase ^= 1u;
   }
   if (abort_flag) {      // a wait was given up: copies in flight land before the shared memory is released
     const long long t0 = clock64();
@@ -401,8 +402,8 @@ struct NormSource {
 };
 template <int KV, typename Source>
 __global__ void __launch_bounds__(1024) rows_e4m3_walk_kernel(const Source src, uint8_t* __restrict__ q, float* __restrict__ scale, int rows, int cols, float eps,
-                                                                int stages, int* error) {
-  rows_e4m3_walk<KV>(src, q, scale, rows, cols, eps, stages, error);
+                                                                int* error) {
+  rows_e4m3_walk<KV>(src, q, scale, rows, cols, eps, error);
 }
 
 template <typename T, int KV>
@@ -500,17 +501,14 @@ template <int KV, typename Source>
 static bool launch_walk(const Source& src, size_t bytes, uint8_t* q, float* scale, int rows, int cols, float eps, cudaStream_t stream) {
   int* error = gemm_tcgen05_error_address();
   const int threads = ((cols / 8 + KV - 1) / KV + 31) / 32 * 32;
-  // Two rows on their way, or four short ones; with more of them, so fewer blocks a processor, 8,192 norms of 4,096 took 56 us for 45.
-  int stages = kRowStages;
-  while (stages > 2 && stages * bytes > 32 * 1024) --stages;
-  const size_t smem = stages * bytes;
+  const size_t smem = kRowStages * bytes;
   if (!error || smem > kWalkSmem) return false;
   const int by_threads = 1024 / ((threads + 127) / 128 * 128), by_smem = (int)((224 * 1024) / (smem + 2048)), blocks = by_threads < by_smem ? by_threads : by_smem;
   auto kernel = rows_e4m3_walk_kernel<KV, Source>;
   static std::atomic<uint64_t> done{0};
   if (smem > 40 * 1024) allow_smem(kernel, kWalkSmem, done);
   const int grid = blocks * processors();
-  launch_kernel(kernel, dim3(rows < grid ? rows : grid), dim3(threads), smem, stream, src, q, scale, rows, cols, eps, stages, error);
+  launch_kernel(kernel, dim3(rows < grid ? rows : grid), dim3(threads), smem, stream, src, q, scale, rows, cols, eps, error);
   return true;
 }
 
