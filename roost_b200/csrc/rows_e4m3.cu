@@ -150,8 +150,8 @@ __device__ void row_e4m3(const Row& row, uint8_t* q, float* scale_out, int cols,
 }
 
 // ---------------------------------------------------------------------------------------------- rows in registers
-// Rows of whole 16-byte pieces: a thread takes KV vectors of eight numbers, all its loads first, and the row stays in registers between the search
-// for its largest number and the rounding: one pass over memory.
+// Rows of whole 16-byte pieces: a thread takes KV vectors of eight numbers, all its loads first, and the row stays in registers (but for some bytes of four
+// vectors) between the search for its largest number and the rounding: one pass over memory.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   if constexpr (sizeof(T) == 2) {
@@ -427,8 +427,10 @@ __global__ void __launch_bounds__(1024) silu_mul_e4m3_vec_kernel(const T* __rest
   row.shift = shift;
   row_e4m3_vec<KV>(row, q + t * inter, scale + t, inter, 0.f);
 }
+// Four vectors a thread want a block's whole 64 registers; not told so, the compiler took 32 for a 32-bit stream and spilled 336 bytes (295 rows of 20,000 33.5 us
+// for 16.2, 8 of 32,768 15.3 for 9.3). Up to 80 bytes still go to memory there.
 template <typename T, typename TR, int KV, bool ADD, bool EARLY>
-__global__ void __launch_bounds__(1024) rms_norm_e4m3_vec_kernel(const T* __restrict__ x, TR* residual, const void* __restrict__ w, uint8_t* __restrict__ q,
+__global__ void __launch_bounds__(1024, KV == 4 ? 1 : 0) rms_norm_e4m3_vec_kernel(const T* __restrict__ x, TR* residual, const void* __restrict__ w, uint8_t* __restrict__ q,
                                          float* __restrict__ scale, T* __restrict__ kept, const int32_t* __restrict__ rows, int hidden, float eps,
                                          int wdtype) {
   pdl_launch_dependents();
