@@ -181,8 +181,7 @@ class RoostEngine:
             raise AdapterError(f"adapter {name!r} is not loaded")
 
     def _idle_adapter(self, name) -> None:
-        slots = self.model.rt.adapters
-        if slots is not None and name in slots.names and slots.names[name] in self.executor.adapter_of.values():
+        if self.model.rt.adapters is not None and self.model.rt.adapters.in_use(name):
             raise AdapterError(f"adapter {name!r} is in use")
 
     def _release(self, request_id) -> None:

@@ -187,6 +187,8 @@ class StepExecutor:
         self.storage = CacheStorage(self.groups, capacities, self.rt.dtype, self.rt.device)
         # request id -> adapter slot of the requests that use one; None for a model without room for adapters
         self.adapter_of: dict | None = {} if getattr(self.rt, "adapters", None) is not None else None
+        if self.adapter_of is not None:
+            self.rt.adapters.executors.add(self)
         self.builder = BatchBuilder(self.rt.device, self.cache, self.adapter_of)
         self.steps_run = 0
         self.last_upload_bytes = 0

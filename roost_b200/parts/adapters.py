@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import json
 import math
+import weakref
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -46,6 +47,7 @@ class AdapterSlots:
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
         self.names: dict = {}        # adapter -> slot
+        self.executors = weakref.WeakSet()     # whose requests use them (``StepExecutor.adapter_of``): several may run one model
         self.beside: list = []       # the projections that were given room since ``keep_only``
 
     def projection(self, out_features: int, in_features: int, widths: tuple | None = None) -> ProjectionAdapters:
@@ -65,6 +67,9 @@ class AdapterSlots:
             if id(part.adapters) not in kept:
                 part.adapters = None
         self.beside = []
+
+    def in_use(self, name) -> bool:
+        return name in self.names and any(self.names[name] in ex.adapter_of.values() for ex in self.executors)
 
     def free_slot(self) -> int:
         for s in range(self.count):
