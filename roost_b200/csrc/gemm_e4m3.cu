@@ -35,29 +35,6 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t tmem_d, uint64_t a_desc, 
                "l"(b_desc), "r"(idesc), "r"(accumulate)
                : "memory");
 }
-__device__ __forceinline__ void commit_pair(uint32_t bar) {
-  const uint16_t mask = 3;  // the barrier at this offset in both CTAs of the pair
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar), "h"(mask) : "memory");
-}
-// The load whose bytes count on a barrier of either CTA of the pair.
-__device__ __forceinline__ void load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c_inner, int c_outer) {
-  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(map)), "r"(cluster_bar), "r"(c_inner), "r"(c_outer)
-               : "memory");
-}
-__device__ __forceinline__ uint32_t rank_in_cluster() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t remote_address(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void arrive_remote(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(addr) : "memory");
-}
 // Every thread of the cluster that has not exited arrives and waits; the threads of a warp need not come together.
 __device__ __forceinline__ void sync_cluster() { asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory"); }
 
@@ -417,7 +394,7 @@ __global__ void __launch_bounds__(192, 2)
       tcgen05_fence_before();
     } else {
       const int rows = min(share, 32), owner = nl / share;
-      const uint32_t to = remote_address(sums_base + (uint32_t)(r * share * NTOK + nl % share * Cfg::kBlock) * 4u, owner), to_bar = remote_address(sums_full, owner);
+      const uint32_t to = mapa_shared(sums_base + (uint32_t)(r * share * NTOK + nl % share * Cfg::kBlock) * 4u, owner), to_bar = mapa_shared(sums_full, owner);
 #pragma unroll
       for (int cb = 0; cb < NTOK; cb += Cfg::kBlock) {
         if (cb < M && ok) {
@@ -600,7 +577,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
   auto acc_full = [&](int a) { return bar0 + 8u * (2 * kStages + a); };
   auto acc_empty = [&](int a) { return bar0 + 8u * (2 * kStages + 2 + a); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = rank_in_cluster();
+  const uint32_t rank = cluster_ctarank();
   if (threadIdx.x == 0) {
     abort_flag = 0;
     for (int s = 0; s < kStages; ++s) {
@@ -632,7 +609,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint32_t even_full = remote_address(full(0), 0);
+      const uint32_t even_full = mapa_shared(full(0), 0);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -642,8 +619,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
           if (!(ok = mbar_wait_limited(empty(stage), phase ^ 1u, abortp, 1, error))) break;
           const uint32_t sa = smem_base + stage * kStage;
           if (rank == 0) mbar_expect_tx(full(stage), 2 * kStage);
-          load_2d_pair(sa, &tma_q, even_full + 8u * stage, kb * kBlockK, m0);
-          load_2d_pair(sa + kStageA, &tma_w, even_full + 8u * stage, kb * kBlockK, n0);
+          tma_load_2d_pair(sa, &tma_q, even_full + 8u * stage, kb * kBlockK, m0);
+          tma_load_2d_pair(sa + kStageA, &tma_w, even_full + 8u * stage, kb * kBlockK, n0);
           if (++stage == kStages) stage = 0, phase ^= 1u;
         }
       }
@@ -667,15 +644,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             mma_e4m3_pair(tmem + (uint32_t)(acc * BN), a_desc + (uint64_t)(2 * k), b_desc + (uint64_t)(2 * k), idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-          commit_pair(empty(stage));
+          tcgen05_commit_pair(empty(stage));
           if (++stage == kStages) stage = 0, phase ^= 1u;
         }
-        if (ok) commit_pair(acc_full(acc));
+        if (ok) tcgen05_commit_pair(acc_full(acc));
       }
     }
   } else {
     const int lanes = (warp & 3) * 32;
-    const uint32_t even_acc_empty[2] = {remote_address(acc_empty(0), 0), remote_address(acc_empty(1), 0)};
+    const uint32_t even_acc_empty[2] = {mapa_shared(acc_empty(0), 0), mapa_shared(acc_empty(1), 0)};
     int it = 0;
     for (int t = pair; t < tiles; t += pairs, it += chains) {
       const int acc = it & 1, row = (t % m_tiles) * 256 + (int)rank * 128 + lanes, n0 = (t / m_tiles) * 256;
@@ -687,8 +664,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) {
-        arrive_remote(even_acc_empty[acc]);
-        if (chains == 2) arrive_remote(even_acc_empty[1]);
+        mbar_arrive_cluster(even_acc_empty[acc]);
+        if (chains == 2) mbar_arrive_cluster(even_acc_empty[1]);
       }
     }
   }
