@@ -6,8 +6,9 @@
 //   few rows of q: 128 rows of w are the tile's rows and the rows of q its columns, k is split over a cluster (gemm_e4m3_split_kernel);
 //   more: persistent CTAs, one a processor, on tiles of 128 x 64, 128 or 256 (gemm_e4m3_tile_kernel);
 //   many: pairs of CTAs on tiles of 256 x 256 (gemm_e4m3_pair_kernel).
-// Measured: 8 x 4,096 x 4,096 4.8 us, 8 x 24,576 x 4,096 19.3 (5.2 TB/s of w), 128 x 4,096 x 4,096 9.7, 333 x 6,144 x 4,096 14.4, 4,096 x 4,096 x 12,288 139
-// (2.96 PFLOP/s, a library product's rate). In between a block of k bounds it: 0.287 us of a tensor core, whatever the columns up to 128.
+// Measured, random numbers, weights from memory: 8 x 4,096 x 4,096 5.1 us, 8 x 24,576 x 4,096 19.4 (5.2 TB/s of w), 128 x 4,096 x 4,096 10.5, 333 x 6,144 x 4,096
+// 15.3, 4,096 x 4,096 x 12,288 148 in short runs (2.8 PFLOP/s; a library product 143) and 177 to 182 under the power cap (2.3; 165). In between a block of k
+// bounds it: 0.287 us of a tensor core, whatever the columns up to 128.
 // A block of k is 128 numbers, a row of the 128-byte swizzle. Every wait on a barrier has a limit, after which the kernel records a code (read back
 // with those of the bfloat16 products), lets its copies land, frees its tensor memory and returns.
 #include <cuda_fp8.h>
@@ -60,8 +61,8 @@ __device__ __forceinline__ void let_copies_land(volatile int* abortp) {
 constexpr uint32_t kStoreBytes = 4 * 32 * 128;
 // The tensor cores cut their sums off, so a chain of them leans towards zero with its length: 1.3e-6 of the outputs' norm at a k of 14,640, 4e-7 in
 // two chains of half of it that are added to nearest. 16-bit outputs do not see it; float32 outputs of a long k have two chains, in both accumulators of a
-// tile, so that the next tile's products wait for this one's stores: with the stores' twice as many bytes 4,096 x 4,096 x 12,288 takes 170 us, 152 with
-// 16-bit outputs and one chain; 1,000 x 4,096 x 14,336 50 and 46.
+// tile, so that the next tile's products wait for this one's stores: with the stores' twice as many bytes 4,096 x 4,096 x 12,288 takes 170 us, 150 with
+// 16-bit outputs and one chain; 1,000 x 4,096 x 14,336 52 and 50.
 template <typename TOut>
 __host__ __device__ constexpr bool two_chains(int k) { return sizeof(TOut) == 4 && k > 8192; }
 template <typename TOut, int N>
@@ -837,7 +838,8 @@ int launch_any(const Operands& o) {
 
 // The form with the least time by a count of its steps: rounds of tiles over the processors, a block of k each, and what a launch takes beside. A block of k
 // takes as long for 128 columns as for 64 (a product of 128 x 32 from shared memory takes 128 cycles up to there), 0.41 us for 256 and 0.37 for a
-// pair's 256 x 256, measured over 4,096 x 4,096 x 12,288 (385, 193, 155 and 143 us); beside it 512 rows x 4,096 x 4,096 took 3.7, 4.2, 4.1 and 4.4 us more, and
+// pair's 256 x 256, measured over 4,096 x 4,096 x 12,288 in short runs of numbers that toggle
+// little, so that the clock stays up (385, 193, 155 and 143 us); beside it 512 rows x 4,096 x 4,096 took 3.7, 4.2, 4.1 and 4.4 us more, and
 // the split form 7 to 8 (128 x 4,096 x 4,096 9.7 us for 8 blocks, 256 x 4,096 x 12,288 22.7 for 48).
 enum Form { kTile64, kTile128, kTile256, kPair, kSplit };
 Form form_of(int m, int n, int k) {

@@ -637,7 +637,8 @@ int roost_silu_mul_e4m3(const void* x, void* q, float* scale, int tokens, int in
 /* The same, and v rounded once to x's type in kept [tokens, inter] (null: nothing is kept). */
 int roost_silu_mul_e4m3_kept(const void* x, void* q, float* scale, void* kept, int tokens, int inter, int block, int dtype, roost_stream_t stream);
 /* v = rms_norm(s) * w in 32 bits with s = x, or residual + x rounded to residual_dtype (that of x, or float32) where residual is not null; s
- * replaces residual unless `rows` gathers (as roost_add_rms_norm). kept (null, or of x's type): v as the norm without the 8 bits gives it. */
+ * replaces residual unless `rows` gathers (as roost_add_rms_norm). kept (null, or of x's type): v rounded once (the weight's factor comes ahead of
+ * the row's, so a number may be the neighbour of what roost_add_rms_norm gives). */
 int roost_rms_norm_e4m3(const void* x, void* residual, const void* w, void* q, float* scale, void* kept, const int32_t* rows, int n_out, int hidden,
                         float eps, int dtype, int residual_dtype, int wdtype, roost_stream_t stream);
 

@@ -7,8 +7,8 @@
 // value saturates; the least scale keeps a row of zeros from dividing by zero. The search for the largest magnitude keeps an infinity or
 // a NaN: a row that holds either gets a scale that is not finite and numbers that are NaN or meet that scale in the product, so the row of the product
 // is NaN as it would be without the 8 bits, and no other row is touched.
-// Measured: a norm of 8,192 x 4,096 with its residual 42.4 us (5.5 TB/s), 3,001 x 5,120 float32 rows 12.3 (6.2 TB/s), both bound by memory; silu(gate) up of
-// 4,096 x 12,288 46.9 (5.4 TB/s), bound by issue slots, about 30 instructions a number; 8 to 64 rows 1.9 to 2.9, one trip to memory and two exchanges.
+// Measured, in a graph of calls: a norm of 8,192 x 4,096 with its residual 43.0 us (5.5 TB/s), 3,001 x 5,120 float32 rows 12.5 (6.1 TB/s), both bound by memory;
+// silu(gate) up of 4,096 x 12,288 49.8 (5.1 TB/s), bound by issue slots, about 32 instructions a number; 8 to 64 rows 1.8 to 2.9, one trip to memory and two exchanges.
 #include <cuda_fp8.h>
 
 #include "tma.cuh"
@@ -33,7 +33,7 @@ __device__ __forceinline__ float over(float v, float scale, float inv) {
   return fmaf(fmaf(-r, scale, v), inv, r);
 }
 // silu(g) u. The reciprocal is within a unit in its last place, where a quotient would be within half of one: of 7.5e7 numbers 78 are not the one nearest to the
-// formula's, 76 with the quotient, which takes 57 us for 4,096 x 12,288. A quarter of 1 + exp(-g) stands for it, so that the reciprocal is a normal number (others
+// formula's, 76 in PyTorch's 32 bits; with the quotient 4,096 x 12,288 takes 57 us. A quarter of 1 + exp(-g) stands for it, so that the reciprocal is a normal number (others
 // are given as zero) wherever the exponential is finite; that takes 49.9 us for 46.9.
 __device__ __forceinline__ float gated(float g, float u) {
   float r;
