@@ -654,7 +654,7 @@ int roost_gemm_e4m3(const void* q, const float* q_scale, const void* w, const fl
  * slot's rows are used (null: all). rows[0 .. listed): the tokens that have an adapter; tiles [n_tiles][3] = (slot, first, end): the tokens
  * rows[first .. end), at most tile_rows (64 at most), have adapter `slot`; a slot outside [0, slots), a token outside [0, tokens) and what of a range lies outside
  * [0, listed) are passed over, and a tile's tokens beyond tile_rows. A token
- * is listed once at most. y's other rows are left as they are. n_parts <= 8, n_parts * rank <= 512. h: workspace of
+ * is listed once at most, and y shares no numbers with x, a and b. y's other rows are left as they are. n_parts <= 8, n_parts * rank <= 512. h: workspace of
  * roost_adapters_workspace_bytes() bytes (0: none is needed), not shared by calls that may run at the same time. Two launches, or one where the
  * workspace is not used (float32, or rows that are no whole 16-byte pieces). */
 int64_t roost_adapters_workspace_bytes(int listed, int n_parts, int rank, int dtype, int y_dtype);

@@ -543,8 +543,8 @@ class KernelLibrary:
 
     def adapters_add_(self, y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, plan: AdapterPlan,
                       widths: tuple | None = None, ranks: torch.Tensor | None = None) -> torch.Tensor:
-        """y[t] += scale[s] * b[s] (a[s] x[t]) in place for every token t whose request has an adapter s; the other rows of y stay as they are. y: what
-        the shared projection made of x, rows [T, N] that may lie apart, in x's type (or float32 beside bfloat16). ``widths``: the parts of the
+        """y[t] += scale[s] * b[s] (a[s] x[t]) in place for every token t whose request has an adapter s; the other rows of y stay as they are. y (no number of
+        which x, a or b has): what the shared projection made of x, rows [T, N] that may lie apart, in x's type (or float32 beside bfloat16). ``widths``: the parts of the
         projection's outputs (queries, keys and values, say), each with an adapter of its own; None: one part. a [slots, parts, rank, K] and b
         [slots, N, rank] in x's type, scale float32 [slots]; ``ranks`` int32 [slots]: how many of the rank's rows a slot uses (None: all)."""
         here = _need_here("adapters_add_", y, x, a, b, scale, ranks, plan.rows, plan.tiles)
